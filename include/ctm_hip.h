@@ -298,6 +298,27 @@ int ctm_rdm_c4v(ctm_ctx* ctx, int which, const double* a, const double* C, const
  * out is the un-padded, max-abs-normalised tensor of the NEIGHBOUR site `a`. */
 int ctm_init_piece(ctm_ctx* ctx, int kind, const double* a, const int* adims, double* out);
 
+/* ---- the optimiser's operators over a list of tensors (optim/ad_optim_lbfgs_mod.py:132-360: the gradient of all on-site tensors) ------ */
+/* nt tensors of n[i] elements (dense memory in any order of the axes; n[i] = 0 allowed) of the context's dtype, pointers 8-byte aligned.
+ * The pointer arrays live on the HOST and are read during the call.  hip_stream: the stream the kernels are enqueued on (a hipStream_t of the
+ * context's device, NULL = the default stream) -- not the context's own, whose workspace these entries do not touch; no host synchronisation,
+ * no allocation, no memset: a call may be captured into a graph.  ws: caller-owned device memory of at least CTM_GRAD_WS_DOUBLES(nt) doubles,
+ * not shared by calls that may run at the same time; afterwards
+ *     ws[0] = (sum |x|^2)^1/2 over the whole list, no overflow or underflow of the squares        ws[1] = max |x|
+ *     ws[2] = c = 1 if the chosen norm <= max_norm, else max_norm / norm (NaN norm: NaN; infinite norm: 0)
+ * (0, 0, 1 for an empty list; NaN in the list: both NaN).  Sums have a fixed order: equal inputs give equal bits.
+ * Memory that is written must not overlap any other range of the call (clip: y[i] == x[i] is allowed): CTM_ERR_BADARG. */
+#define CTM_GRAD_WS_DOUBLES(nt) (4 * (1025 + (nt)))
+enum { CTM_NORM_INF = 0, CTM_NORM_2 = 2 };
+int ctm_grad_norms(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x, const long long* n, double* ws, long long ws_doubles);
+/* y[i] = c x[i]; in place (y[i] == x[i]) a list inside the bound keeps its bits */
+int ctm_grad_clip(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x, double* const* y, const long long* n, int norm_type,
+                  double max_norm, double* ws, long long ws_doubles);
+/* g' = c g (c = 1 and ws unused for max_norm < 0);  m <- g' (first != 0) or momentum m + (1 - dampening) g';  p <- p - lr m.
+ * m NULL (momentum 0): p <- p - lr g'.  g is not written. */
+int ctm_sgd_step(ctm_ctx* ctx, void* hip_stream, int nt, double* const* p, const double* const* g, double* const* m, const long long* n,
+                 double lr, double momentum, double dampening, int first, int norm_type, double max_norm, double* ws, long long ws_doubles);
+
 #ifdef __cplusplus
 }
 #endif

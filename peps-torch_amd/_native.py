@@ -100,6 +100,11 @@ _SIGS = {
     "ctm_rdm1x2": [C.c_void_p, C.POINTER(C.c_void_p), C.c_int, C.POINTER(C.c_int), C.c_void_p],
     "ctm_rdm_c4v": [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p],
     "ctm_init_piece": [C.c_void_p, C.c_int, C.c_void_p, C.POINTER(C.c_int), C.c_void_p],
+    "ctm_grad_norms": [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_longlong), C.c_void_p, C.c_longlong],
+    "ctm_grad_clip": [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_longlong), C.c_int, C.c_double,
+                      C.c_void_p, C.c_longlong],
+    "ctm_sgd_step": [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_longlong),
+                     C.c_double, C.c_double, C.c_double, C.c_int, C.c_int, C.c_double, C.c_void_p, C.c_longlong],
     "ctm_move": [C.c_void_p, C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_int, C.POINTER(MoveUnit), C.c_int, C.POINTER(TruncCfg), C.c_int, C.c_int],
 }
 EXPORTS = sorted(list(_SIGS) + ["ctm_last_error", "ctm_version"])
@@ -150,6 +155,30 @@ def _plain(t):
     if t.is_neg():
         t = t.resolve_neg()
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _is_dense(t):
+    """The elements fill one range of memory, in whatever order of the axes."""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for st, m in sorted((st, m) for st, m in zip(t.stride(), t.shape) if m > 1):
+        if st != n:
+            return False
+        n *= m
+    return True
+
+
+def _put_back(pairs):
+    if pairs:
+        with torch.no_grad():
+            for t, v in pairs:
+                t.copy_(v)
+
+
+def _changed(tensors):
+    """Tell autograd that the library wrote these tensors: a backward pass that saved one of them must notice."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 class Engine:
@@ -875,6 +904,164 @@ class Engine:
         out = self.empty(*[a.shape[k] ** 2 for k in kept])
         self._ck(self.lib.ctm_init_piece(self.h, kind, _ptr(a), self._adims(a), _ptr(out)), "init_piece")
         return out
+
+    # ---- the optimiser's operators over a list of tensors -----------------------------------------
+    # They run on the CALLER's current stream (torch's rule for its own operators) and bring their workspace along from torch's allocator, so
+    # that two of them may be under way on two streams and a captured one owns its workspace.
+    def _list(self, what, tensors):
+        """The tensors of a list, checked: device tensors of this engine's device and of one dtype, holding the values themselves."""
+        ts = list(tensors)
+        dt, dev = (ts[0].dtype if ts and isinstance(ts[0], torch.Tensor) else torch.float64), self.device
+        for i, t in enumerate(ts):
+            if not isinstance(t, torch.Tensor):
+                raise NativeError(f"{what}: element {i} is {type(t)}, not a tensor")
+            if t.device != dev:
+                raise NativeError(f"{what}: tensor {i} is on {t.device}, the engine on {dev}: use _native.engine(tensor.device)")
+            if t.dtype is not dt or dt not in _DTYPES:
+                raise NativeError(f"{what}: tensor {i} has dtype {t.dtype}: all tensors of a list have the same dtype, float64 or complex128")
+            if t.layout is not torch.strided:
+                raise NativeError(f"{what}: tensor {i} is not a dense (strided) tensor")
+        return ts, dt
+
+    @staticmethod
+    def _same_lists(what, a, b, name):
+        if len(a) != len(b):
+            raise NativeError(f"{what}: {len(a)} tensors, but {len(b)} {name}")
+        for i, (x, y) in enumerate(zip(a, b)):
+            if x.shape != y.shape or x.dtype is not y.dtype:
+                raise NativeError(f"{what}: {name} {i} is {tuple(y.shape)} {y.dtype}, its tensor {tuple(x.shape)} {x.dtype}")
+
+    @staticmethod
+    def _written(what, outs):
+        """Tensors that a call writes: memory of their own, every element of its own, holding the values themselves.  (The library compares the
+        ranges of contiguous tensors; here the extents, where one of the tensors is a strided view.)"""
+        views = False
+        for i, t in enumerate(outs):
+            if t.is_conj() or t.is_neg():
+                raise NativeError(f"{what}: tensor {i} is a lazily conjugated or negated view: it cannot be written")
+            if not t.is_contiguous():
+                views = True
+                span = 1
+                for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+                    if st < span:
+                        raise NativeError(f"{what}: elements of tensor {i} share memory (strides {t.stride()}): it cannot be written")
+                    span += st * (n - 1)
+        if views:
+            end = 0
+            for a, b in sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))))
+                               for t in outs if t.numel()):
+                if a < end:
+                    raise NativeError(f"{what}: the extents of two tensors that are written overlap")
+                end = b
+
+    @staticmethod
+    def _ptrs(ts):
+        return (C.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
+
+    def _run_lists(self, what, dt, fn):
+        """fn(handle, stream) with this engine's device current and the calling thread's current stream of it."""
+        def call():
+            self._bind_dtype(dt)
+            self._ck(fn(self.h, C.c_void_p(torch._C._cuda_getCurrentRawStream(self.device.index))), what)
+        if torch.cuda.current_device() == self.device.index:
+            call()
+        else:
+            with torch.cuda.device(self.device):
+                call()
+
+    def _grad_ws(self, nt):
+        return torch.empty(4 * (1025 + nt), dtype=torch.float64, device=self.device)          # CTM_GRAD_WS_DOUBLES(nt)
+
+    @staticmethod
+    def _norm_code(what, norm_type):
+        if norm_type == 2:
+            return 2
+        if norm_type == float("inf"):
+            return 0
+        raise NativeError(f"{what}: norm_type {norm_type!r}: 2 or inf")
+
+    @staticmethod
+    def _max_norm(what, max_norm):
+        max_norm = float(max_norm)
+        if not max_norm >= 0.0:
+            raise NativeError(f"{what}: max_norm {max_norm}: a bound >= 0")
+        return max_norm
+
+    def grad_norms(self, tensors):
+        """[2-norm, largest modulus] of all elements of a list of tensors: float64 device tensor of two elements."""
+        ts, dt = self._list("grad_norms", tensors)
+        xs = [t if _is_dense(t) else t.contiguous() for t in ts]           # (any order of the elements; a conjugate has the same norms)
+        ws = self._grad_ws(len(xs))
+        n = (C.c_longlong * len(xs))(*[t.numel() for t in xs])
+        self._run_lists("grad_norms", dt, lambda h, s: self.lib.ctm_grad_norms(h, s, len(xs), self._ptrs(xs), n, _ptr(ws), ws.numel()))
+        return ws[:2]
+
+    def clip_grads(self, tensors, max_norm, norm_type=2, out=None):
+        """Scale a list of tensors by c = min(1, max_norm / norm), norm = 2-norm or largest modulus (norm_type inf) of the WHOLE list: in place,
+        or into the tensors `out`.  Returns [2-norm, largest modulus] of the unscaled list."""
+        what = "clip_grads"
+        code, max_norm = self._norm_code(what, norm_type), self._max_norm(what, max_norm)
+        ts, dt = self._list(what, tensors)
+        if out is None:
+            outs = ts
+        else:
+            outs, _ = self._list(what, out)
+            self._same_lists(what, ts, outs, "outputs")
+        self._written(what, outs)
+        xs, ys, back = [], [], []
+        for i, (x, y) in enumerate(zip(ts, outs)):
+            if not (x is y and _is_dense(x)):
+                x = _plain(x)
+                if not y.is_contiguous():
+                    back.append(i)
+                    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+            xs.append(x)
+            ys.append(y)
+        ws = self._grad_ws(len(xs))
+        n = (C.c_longlong * len(xs))(*[t.numel() for t in xs])
+        self._run_lists(what, dt, lambda h, s: self.lib.ctm_grad_clip(h, s, len(xs), self._ptrs(xs), self._ptrs(ys), n, code, max_norm, _ptr(ws),
+                                                                      ws.numel()))
+        _put_back([(outs[i], ys[i]) for i in back])
+        _changed(outs)
+        return ws[:2]
+
+    def sgd_step(self, params, grads, bufs=None, lr=1.0, momentum=0.0, dampening=0.0, first=False, max_norm=None, norm_type=2):
+        """One step of gradient descent with momentum on a list of tensors, in place:  g' = c g,  m <- g' (first) or momentum m + (1 - dampening) g',
+        p <- p - lr m;  without momentum (bufs is not read) p <- p - lr g'.  c = 1 without `max_norm`, else the factor of clip_grads for the
+        list `grads`, whose tensors are not written.  Returns [2-norm, largest modulus] of `grads`, or None without `max_norm`."""
+        what = "sgd_step"
+        code = self._norm_code(what, norm_type)
+        bound = -1.0 if max_norm is None else self._max_norm(what, max_norm)
+        lr, momentum, dampening = float(lr), float(momentum), float(dampening)
+        if not (lr >= 0.0 and momentum >= 0.0):
+            raise NativeError(f"{what}: lr {lr}, momentum {momentum}: both >= 0")
+        ps, dt = self._list(what, params)
+        gs, _ = self._list(what, grads)
+        self._same_lists(what, ps, gs, "gradients")
+        ms = None
+        if momentum != 0.0:
+            if bufs is None:
+                raise NativeError(f"{what}: momentum needs the momentum buffers")
+            ms, _ = self._list(what, bufs)
+            self._same_lists(what, ps, ms, "momentum buffers")
+        self._written(what, ps if ms is None else ps + ms)
+        wp, wg, wm, back = [], [], [], []
+        for i, (p, g) in enumerate(zip(ps, gs)):
+            m = ms[i] if ms is not None else p
+            if p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and not g.is_conj() and not g.is_neg():
+                wp.append(p); wg.append(g); wm.append(m)
+            else:
+                back.append(i)
+                wp.append(p.detach().clone(memory_format=torch.contiguous_format)); wg.append(_plain(g))
+                wm.append(m.detach().clone(memory_format=torch.contiguous_format))
+        ws = self._grad_ws(len(ps)) if bound >= 0.0 else None
+        n = (C.c_longlong * len(ps))(*[t.numel() for t in ps])
+        self._run_lists(what, dt, lambda h, s: self.lib.ctm_sgd_step(h, s, len(ps), self._ptrs(wp), self._ptrs(wg), None if ms is None else self._ptrs(wm),
+                                                                     n, lr, momentum, dampening, int(first), code, bound,
+                                                                     None if ws is None else _ptr(ws), 0 if ws is None else ws.numel()))
+        _put_back([(ps[i], wp[i]) for i in back] + ([] if ms is None else [(ms[i], wm[i]) for i in back]))
+        _changed(ps if ms is None else ps + ms)
+        return None if ws is None else ws[:2]
 
 
 _engines = {}

@@ -10,8 +10,10 @@ import os, subprocess, sys, shutil
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
-SOURCES = ["ctm_runtime.hip", "gemm_f64.hip", "tensor_ops.hip", "jacobi_core.hip", "svd_leading.hip", "eigh.hip", "contract.hip", "layer2.hip", "ctm_ops.hip", "backward.hip", "ctm_move.hip"]
+SOURCES = ["ctm_runtime.hip", "gemm_f64.hip", "tensor_ops.hip", "jacobi_core.hip", "svd_leading.hip", "eigh.hip", "contract.hip", "layer2.hip", "ctm_ops.hip", "backward.hip", "ctm_move.hip", "grads.hip"]
 HEADERS = ["ctm_common.h", "contract.h", "jacobi_internal.h", os.path.join("..", "..", "include", "ctm_hip.h")]
+# no packed single-precision arithmetic (v_pk_*_f32): some of its forms have given wrong results on this hardware
+FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 LIB = os.path.join(PKG, "libctm_hip.so")
 LIB_ASAN = os.path.join(PKG, "libctm_hip_asan.so")
 
@@ -47,7 +49,7 @@ def build(force=False, verbose=True, asan=False):
         o = os.path.join(objdir, os.path.basename(s).replace(".hip", ".o"))
         objs.append(o)
         if force or not os.path.exists(o) or any(os.path.getmtime(o) < os.path.getmtime(d) for d in [s] + deps[len(srcs):]):
-            cmd = [cc, "--offload-arch=gfx950"] + opt + ["-std=c++17", "-fPIC", "-c", s, "-o", o]
+            cmd = [cc, "--offload-arch=gfx950"] + opt + FP32 + ["-std=c++17", "-fPIC", "-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((cmd, subprocess.Popen(cmd)))

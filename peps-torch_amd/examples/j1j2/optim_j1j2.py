@@ -14,7 +14,7 @@ from ipeps.ipeps import IPEPS, read_ipeps, extend_bond_dim
 from ctm.generic.env import ENV, init_env, ctmrg_conv_specC
 from ctm.generic import ctmrg, transferops
 from models import j1j2
-from optim.ad_optim_lbfgs_mod import optimize_state
+from optim import ad_optim_lbfgs_mod, ad_optim_sgd_mod
 
 log = logging.getLogger(__name__)
 
@@ -27,6 +27,7 @@ parser.add_argument("--hz_stag", type=float, default=0., help="staggered mag. fi
 parser.add_argument("--h_uni", nargs=3, type=float, default=[0, 0, 0], help="uniform mag. field with components in directions h^z, h^x, h^y")
 parser.add_argument("--delta_zz", type=float, default=1., help="easy-axis (nearest-neighbour) anisotropy")
 parser.add_argument("--tiling", default="BIPARTITE", help="tiling of the lattice", choices=["BIPARTITE", "1SITE", "2SITE", "4SITE", "8SITE"])
+parser.add_argument("--optimizer", default="lbfgs", help="optimisation of the state", choices=["lbfgs", "sgd"])
 parser.add_argument("--top_freq", type=int, default=-1, help="frequency of transfer operator spectrum evaluation")
 parser.add_argument("--top_n", type=int, default=2, help="number of leading eigenvalues of transfer operator to compute")
 parser.add_argument("--ctm_conv_crit", default="CSPEC", help="ctm convergence criterion", choices=["CSPEC", "ENERGY"])
@@ -129,7 +130,8 @@ def main(args=None):
                     l = transferops.get_Top_spec(args.top_n, c, d, state, ctm_env)
                     print("TOP " + json.dumps(_to_json(l)))
 
-    optimize_state(state, ctm_env, loss_fn, obs_fn=obs_fn)
+    optim_mod = ad_optim_sgd_mod if args.optimizer == "sgd" else ad_optim_lbfgs_mod
+    optim_mod.optimize_state(state, ctm_env, loss_fn, obs_fn=obs_fn)
 
     # final observables of the best variational state
     outputstatefile = args.out_prefix + "_state.json"

@@ -13,7 +13,7 @@ from ctm.one_site_c4v.env_c4v import ENV_C4V, init_env
 from ctm.one_site_c4v import ctmrg_c4v, transferops_c4v
 from ctm.one_site_c4v.rdm_c4v import rdm2x1_sl
 from models import j1j2
-from optim.ad_optim_lbfgs_mod import optimize_state
+from optim import ad_optim_lbfgs_mod, ad_optim_sgd_mod
 
 parser = cfg.get_args_parser()
 parser.add_argument("--j1", type=float, default=1., help="nearest-neighbour coupling")
@@ -22,6 +22,7 @@ parser.add_argument("--j3", type=float, default=0., help="next-to-next nearest-n
 parser.add_argument("--hz_stag", type=float, default=0., help="staggered mag. field")
 parser.add_argument("--h_uni", nargs=3, type=float, default=[0, 0, 0], help="uniform mag. field with components in directions h^z, h^x, h^y")
 parser.add_argument("--delta_zz", type=float, default=1., help="easy-axis (nearest-neighbour) anisotropy")
+parser.add_argument("--optimizer", default="lbfgs", help="optimisation of the state", choices=["lbfgs", "sgd"])
 parser.add_argument("--top_freq", type=int, default=-1, help="frequency of transfer operator spectrum evaluation")
 parser.add_argument("--top_n", type=int, default=2, help="number of leading eigenvalues of transfer operator to compute")
 parser.add_argument("--force_cpu", action='store_true', help="accepted for compatibility; the energy is evaluated on the GPU")
@@ -108,7 +109,8 @@ def main(args=None):
             l = transferops_c4v.get_Top_spec_c4v(args.top_n, state_sym, ctm_env)
             print("TOP " + json.dumps(_to_json(l)))
 
-    optimize_state(state, ctm_env, loss_fn, obs_fn=obs_fn)
+    optim_mod = ad_optim_sgd_mod if args.optimizer == "sgd" else ad_optim_lbfgs_mod
+    optim_mod.optimize_state(state, ctm_env, loss_fn, obs_fn=obs_fn)
 
     # final observables of the best variational state
     outputstatefile = args.out_prefix + "_state.json"

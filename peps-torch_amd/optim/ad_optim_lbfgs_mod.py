@@ -14,6 +14,7 @@ import time
 import torch
 import config as cfg
 import parallel
+from optim import grads
 
 log = logging.getLogger(__name__)
 
@@ -34,6 +35,9 @@ def create_optimizer(state, main_args=cfg.main_args, opt_args=cfg.opt_args, ctm_
     ls = opt_args.line_search
     if ls not in (None, "default", "strong_wolfe", "backtracking"):
         raise RuntimeError("unsupported line search")
+    if opt_args.clip_grad_norm > 0.0 and ls in ("strong_wolfe", "backtracking"):
+        # the search compares the loss along the step with the slope: a scaled gradient is not that slope
+        raise RuntimeError("clip_grad_norm needs the fixed step (line_search default)")
     optimizer = torch.optim.LBFGS(parameters, max_iter=opt_args.max_iter_per_epoch, lr=opt_args.lr,
                                   tolerance_grad=opt_args.tolerance_grad, tolerance_change=opt_args.tolerance_change,
                                   history_size=opt_args.history_size, line_search_fn="strong_wolfe" if ls == "strong_wolfe" else None)
@@ -49,6 +53,8 @@ def load_optimizer_state_(optimizer, state, main_args=cfg.main_args, opt_args=cf
     checkpoint = torch.load(main_args.opt_resume, map_location=state.device, weights_only=False)
     sd = checkpoint["optimizer_state_dict"]
     group = sd["param_groups"][0]
+    if "history_size" not in group:
+        raise RuntimeError(f"{main_args.opt_resume} is not a checkpoint of L-BFGS")
     hist = sd["state"][group["params"][0]]
     if main_args.opt_resume_override_params:
         group.update(lr=opt_args.lr, max_iter=opt_args.max_iter_per_epoch, tolerance_grad=opt_args.tolerance_grad,
@@ -64,6 +70,15 @@ def load_optimizer_state_(optimizer, state, main_args=cfg.main_args, opt_args=cf
         group["history_size"] = opt_args.history_size
     optimizer.load_state_dict(sd)
     print(f"checkpoint.loss = {checkpoint['loss']}")
+
+
+def _grad_norms(gs):
+    """[2-norm, largest modulus] of all gradients, on the host.  (Tensors that the engine does not take -- a run on an engine double on the
+    host, sites of different dtypes -- go through torch.)"""
+    if all(g.is_cuda and g.dtype is gs[0].dtype for g in gs) and gs[0].dtype in (torch.float64, torch.complex128):
+        return grads.grad_norms(gs).tolist()
+    flat = torch.cat(tuple(g.reshape(-1) for g in gs))
+    return [flat.norm().item(), flat.abs().max().item()]
 
 
 def _armijo(phi, phi0, derphi0, c1=1e-4, alpha0=1.0, amin=1.0e-8):
@@ -90,10 +105,12 @@ def _armijo(phi, phi0, derphi0, c1=1e-4, alpha0=1.0, amin=1.0e-8):
 
 
 def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, main_args=cfg.main_args, opt_args=cfg.opt_args,
-                   ctm_args=cfg.ctm_args, global_args=cfg.global_args):
+                   ctm_args=cfg.ctm_args, global_args=cfg.global_args, create=create_optimizer, load=load_optimizer_state_):
     """Minimise `loss_fn(state, env, opt_context) -> (loss, env, history, t_ctm, t_obs[, t_loss])` over the on-site tensors of
     `state`.  Every evaluation starts from the environment the previous one returned (detached); the lowest-loss state is written
-    to `<out_prefix>_state.json`, a checkpoint before every step to `<out_prefix>_checkpoint.p`."""
+    to `<out_prefix>_state.json`, a checkpoint before every step to `<out_prefix>_checkpoint.p`.  `create` / `load` make and restore the
+    optimiser (ad_optim_sgd_mod: gradient descent).  `opt_args.clip_grad_norm` > 0 bounds the 2-norm of the gradient that reaches it; the log
+    and the `tolerance_grad` test see the gradient itself."""
     verbosity = opt_args.verbosity_opt_epoch
     checkpoint_file = main_args.out_prefix + "_checkpoint.p"
     outputstatefile = main_args.out_prefix + "_state.json"
@@ -101,10 +118,12 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
     current_env = [ctm_env_init]
     context = dict({"ctm_args": ctm_args, "opt_args": opt_args, "loss_history": t_data})
     epoch = 0
-    parameters, optimizer = create_optimizer(state, main_args=main_args, opt_args=opt_args, ctm_args=ctm_args, global_args=global_args)
+    parameters, optimizer = create(state, main_args=main_args, opt_args=opt_args, ctm_args=ctm_args, global_args=global_args)
     if main_args.opt_resume is not None:
-        load_optimizer_state_(optimizer, state, main_args=main_args, opt_args=opt_args, ctm_args=ctm_args, global_args=global_args)
+        load(optimizer, state, main_args=main_args, opt_args=opt_args, ctm_args=ctm_args, global_args=global_args)
     calls = [0]
+    clip = opt_args.clip_grad_norm if isinstance(optimizer, torch.optim.LBFGS) else 0.0        # (gradient descent scales inside its step)
+    raw_norms = [None]                                                                         # of the last gradient, where it was scaled in place
 
     def _write_best():
         if parallel.world()[0] == 0:        # replicated run: one writer
@@ -135,17 +154,20 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
         t0 = time.perf_counter()
         loss.backward()
         parallel.average_grads(parameters)             # no-op in a single process; distributed runs: mean of the ranks' local gradients
+        if opt_args.opt_logging and opt_args.opt_log_grad:
+            grad_log = [torch.view_as_real(p.grad).tolist() if p.grad.is_complex() else p.grad.tolist() for p in parameters]
+        if clip > 0.0:
+            raw_norms[0] = grads.clip_grad_norm_(parameters, clip).tolist()
         t1 = time.perf_counter()
         current_env[0] = ctm_env.detach()
         _record(loss.item(), linesearching)
         if opt_args.opt_logging:
-            flat_grad = torch.cat(tuple(p.grad.reshape(-1) for p in parameters))
             entry = dict({"id": epoch, "loss": t_data["loss_ls" if linesearching else "loss"][-1], "t_ctm": t_ctm, "t_check": t_check,
-                          "t_grad": t1 - t0, "grad_mag": [flat_grad.norm().item(), flat_grad.abs().max().item()]})
+                          "t_grad": t1 - t0, "grad_mag": raw_norms[0] if clip > 0.0 else _grad_norms([p.grad for p in parameters])})
             if linesearching:
                 entry["LS"] = len(t_data["loss_ls"])
             if opt_args.opt_log_grad:
-                entry["grad"] = [torch.view_as_real(p.grad).tolist() if p.grad.is_complex() else p.grad.tolist() for p in parameters]
+                entry["grad"] = grad_log
             log.info(json.dumps(entry))
         context['id'] = epoch
         if obs_fn is not None:
@@ -225,10 +247,10 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
             post_proc(state, current_env[0], context)
         if len(t_data["loss"]) > 1 and abs(t_data["loss"][-1] - t_data["loss"][-2]) < opt_args.tolerance_change:
             break
-        flat_grad = torch.cat(tuple(p.grad.reshape(-1) for p in parameters if p.grad is not None))
-        if flat_grad.numel() and flat_grad.abs().max() <= opt_args.tolerance_grad:
+        gs = [p.grad for p in parameters if p.grad is not None and p.grad.numel()]
+        if gs and (raw_norms[0] if clip > 0.0 else _grad_norms(gs))[1] <= opt_args.tolerance_grad:
             break
-        st = optimizer.state[optimizer._params[0]]
+        st = optimizer.state.get(parameters[0], {})
         if 'd' in st and st['d'].mul(st['t']).abs().max() <= opt_args.tolerance_change:
             break
     if len(t_data["loss"]) > 0:

@@ -1,0 +1,93 @@
+"""Gradient descent with momentum on an iPEPS (reference optim/ad_optim_sgd_mod.py): `optimize_state` with the interface, the log, the
+checkpoints and the stopping rules of ad_optim_lbfgs_mod.optimize_state, OPTARGS.lr / momentum / dampening, and a bound on the norm of the
+gradient, OPTARGS.clip_grad_norm.  The update of all on-site tensors, the scaling included, is one call of the native engine
+(optim.grads.sgd_step)."""
+import torch
+import config as cfg
+from optim import ad_optim_lbfgs_mod, grads
+
+
+class SGD(torch.optim.Optimizer):
+    """torch.optim.SGD's iteration (lr, momentum, dampening) with the gradient scaled to 2-norm (or largest modulus, norm_type inf) at most `max_norm`
+    over all parameters; `.grad` is not changed.  `norms` of the last step: device tensor [2-norm, largest modulus] of the raw gradient, None
+    without `max_norm`.  One parameter group, whose lr, momentum, dampening and max_norm may be changed between steps; a graph that captured
+    a step keeps those of the capture, and is captured after the first step (which makes the momentum buffers)."""
+
+    def __init__(self, params, lr, momentum=0.0, dampening=0.0, max_norm=None, norm_type=2):
+        for k, v in (("lr", lr), ("momentum", momentum), ("max_norm", 0.0 if max_norm is None else max_norm)):
+            if not v >= 0.0:
+                raise ValueError(f"invalid {k}: {v}")
+        if norm_type not in (2, float("inf")):
+            raise ValueError(f"invalid norm_type: {norm_type}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, dampening=dampening, max_norm=max_norm, norm_type=norm_type))
+        if len(self.param_groups) != 1:
+            raise ValueError("SGD: one parameter group only (the norm is that of all parameters)")
+        self.norms = None
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        group = self.param_groups[0]
+        ps = [p for p in group["params"] if p.grad is not None]
+        gs = [p.grad for p in ps]
+        kw = dict(lr=group["lr"], momentum=group["momentum"], dampening=group["dampening"])
+        bound = dict(max_norm=group["max_norm"], norm_type=group["norm_type"])
+        if group["momentum"] == 0.0:
+            self.norms = grads.sgd_step(ps, gs, **kw, **bound)
+            return loss
+        new = [p for p in ps if "momentum_buffer" not in self.state[p]]
+        for p in new:
+            self.state[p]["momentum_buffer"] = torch.empty_like(p)
+        bufs = [self.state[p]["momentum_buffer"] for p in ps]
+        if len(new) in (0, len(ps)):
+            self.norms = grads.sgd_step(ps, gs, bufs, first=len(new) > 0, **kw, **bound)
+            return loss
+        # some parameters take their first step, the others do not: two calls, the factor is that of all gradients
+        self.norms = None
+        if bound["max_norm"] is not None:
+            scaled = [torch.empty_like(g) for g in gs]
+            self.norms = grads.clip_grads(gs, out=scaled, **bound)
+            gs = scaled
+        for first in (False, True):
+            part = [i for i, p in enumerate(ps) if any(p is q for q in new) == first]
+            grads.sgd_step([ps[i] for i in part], [gs[i] for i in part], [bufs[i] for i in part], first=first, **kw)
+        return loss
+
+
+def create_optimizer(state, main_args=cfg.main_args, opt_args=cfg.opt_args, ctm_args=cfg.ctm_args, global_args=cfg.global_args):
+    parameters = list(state.get_parameters())
+    for A in parameters:
+        A.requires_grad_(True)
+    if opt_args.line_search not in (None, "default"):
+        raise RuntimeError("unsupported line search")
+    optimizer = SGD(parameters, lr=opt_args.lr, momentum=opt_args.momentum, dampening=opt_args.dampening,
+                    max_norm=opt_args.clip_grad_norm if opt_args.clip_grad_norm > 0.0 else None)
+    optimizer.zero_grad()
+    return parameters, optimizer
+
+
+def load_optimizer_state_(optimizer, state, main_args=cfg.main_args, opt_args=cfg.opt_args, ctm_args=cfg.ctm_args,
+                          global_args=cfg.global_args):
+    """Resume from `main_args.opt_resume`; with `opt_resume_override_params` the stored lr, momentum, dampening and bound are replaced by the
+    current OPTARGS."""
+    print(f"INFO: resuming from check point. resume = {main_args.opt_resume}")
+    checkpoint = torch.load(main_args.opt_resume, map_location=state.device, weights_only=False)
+    sd = checkpoint["optimizer_state_dict"]
+    group = sd["param_groups"][0]
+    if "dampening" not in group:
+        raise RuntimeError(f"{main_args.opt_resume} is not a checkpoint of gradient descent")
+    if main_args.opt_resume_override_params:
+        group.update(lr=opt_args.lr, momentum=opt_args.momentum, dampening=opt_args.dampening,
+                     max_norm=opt_args.clip_grad_norm if opt_args.clip_grad_norm > 0.0 else None)
+    optimizer.load_state_dict(sd)
+    print(f"checkpoint.loss = {checkpoint['loss']}")
+
+
+def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, main_args=cfg.main_args, opt_args=cfg.opt_args,
+                   ctm_args=cfg.ctm_args, global_args=cfg.global_args):
+    """ad_optim_lbfgs_mod.optimize_state with gradient descent in the place of L-BFGS: one evaluation and one step per epoch."""
+    ad_optim_lbfgs_mod.optimize_state(state, ctm_env_init, loss_fn, obs_fn=obs_fn, post_proc=post_proc, main_args=main_args, opt_args=opt_args,
+                                      ctm_args=ctm_args, global_args=global_args, create=create_optimizer, load=load_optimizer_state_)
