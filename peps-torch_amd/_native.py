@@ -132,6 +132,15 @@ def load_library(path=None):
     return lib
 
 
+def load_lists():
+    """The module that reads lists of tensors (csrc/lists.cpp); raises NativeError when it is not there."""
+    try:
+        import _ctm_lists
+    except ImportError as e:
+        raise NativeError(f"{os.path.join(_HERE, '_ctm_lists.so')} is missing or does not load ({e}): build it with `python peps-torch_amd/csrc/build.py`")
+    return _ctm_lists
+
+
 def _ptr(t):
     return C.c_void_p(t.data_ptr())
 
@@ -169,6 +178,10 @@ def _is_dense(t):
     return True
 
 
+def _sequence(x):
+    return x if type(x) in (list, tuple) else list(x)
+
+
 def _put_back(pairs):
     if pairs:
         with torch.no_grad():
@@ -196,6 +209,8 @@ class Engine:
         self._options = {}
         self._tls = threading.local()          # the context selected by _bind is per CALLING THREAD (h, dtype below)
         self._create_lock = threading.Lock()
+        self._lists = load_lists()
+        self._entries = {n: C.cast(getattr(self.lib, "ctm_" + n), C.c_void_p).value for n in ("grad_norms", "grad_clip", "sgd_step")}
         self.workers = []          # engines spawned for concurrent units (units.UnitPool): options/stats fan out to them
         self.default_cfg = TruncCfg(1e-8, 1e-8, 1e-14, 1, 1)
         self._bind_dtype(torch.float64)
@@ -908,6 +923,24 @@ class Engine:
     # ---- the optimiser's operators over a list of tensors -----------------------------------------
     # They run on the CALLER's current stream (torch's rule for its own operators) and bring their workspace along from torch's allocator, so
     # that two of them may be under way on two streams and a captured one owns its workspace.
+    _lists = None
+
+    def _stream(self):
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def _short(self, what, name, tensors, *args):
+        """The call through csrc/lists.cpp, which takes lists of contiguous tensors; None: the general way (the methods below)."""
+        if self._lists is None:
+            return None
+        h = self._handles
+        a, b = h.get(torch.float64), h.get(torch.complex128)
+        r = getattr(self._lists, name)(self._entries[name], 0 if a is None else a.value, 0 if b is None else b.value, self.device, self._stream(),
+                                       tensors, *args)
+        if type(r) is int:
+            self._bind_dtype(tensors[0].dtype)
+            self._ck(r, what)
+        return r
+
     def _list(self, what, tensors):
         """The tensors of a list, checked: device tensors of this engine's device and of one dtype, holding the values themselves."""
         ts = list(tensors)
@@ -962,7 +995,7 @@ class Engine:
         """fn(handle, stream) with this engine's device current and the calling thread's current stream of it."""
         def call():
             self._bind_dtype(dt)
-            self._ck(fn(self.h, C.c_void_p(torch._C._cuda_getCurrentRawStream(self.device.index))), what)
+            self._ck(fn(self.h, C.c_void_p(self._stream())), what)
         if torch.cuda.current_device() == self.device.index:
             call()
         else:
@@ -989,6 +1022,10 @@ class Engine:
 
     def grad_norms(self, tensors):
         """[2-norm, largest modulus] of all elements of a list of tensors: float64 device tensor of two elements."""
+        tensors = _sequence(tensors)
+        r = self._short("grad_norms", "grad_norms", tensors)
+        if r is not None:
+            return r
         ts, dt = self._list("grad_norms", tensors)
         xs = [t if _is_dense(t) else t.contiguous() for t in ts]           # (any order of the elements; a conjugate has the same norms)
         ws = self._grad_ws(len(xs))
@@ -1001,6 +1038,10 @@ class Engine:
         or into the tensors `out`.  Returns [2-norm, largest modulus] of the unscaled list."""
         what = "clip_grads"
         code, max_norm = self._norm_code(what, norm_type), self._max_norm(what, max_norm)
+        tensors, out = _sequence(tensors), None if out is None else _sequence(out)
+        r = self._short(what, "grad_clip", tensors, out, code, max_norm)
+        if r is not None:
+            return r
         ts, dt = self._list(what, tensors)
         if out is None:
             outs = ts
@@ -1035,6 +1076,12 @@ class Engine:
         lr, momentum, dampening = float(lr), float(momentum), float(dampening)
         if not (lr >= 0.0 and momentum >= 0.0):
             raise NativeError(f"{what}: lr {lr}, momentum {momentum}: both >= 0")
+        params, grads = _sequence(params), _sequence(grads)
+        bufs = _sequence(bufs) if momentum != 0.0 and bufs is not None else None
+        if momentum == 0.0 or bufs is not None:
+            r = self._short(what, "sgd_step", params, grads, bufs, lr, momentum, dampening, bool(first), code, bound)
+            if r is not None:
+                return None if r is True else r
         ps, dt = self._list(what, params)
         gs, _ = self._list(what, grads)
         self._same_lists(what, ps, gs, "gradients")

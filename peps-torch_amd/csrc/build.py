@@ -12,6 +12,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 SOURCES = ["ctm_runtime.hip", "gemm_f64.hip", "tensor_ops.hip", "jacobi_core.hip", "svd_leading.hip", "eigh.hip", "contract.hip", "layer2.hip", "ctm_ops.hip", "backward.hip", "ctm_move.hip", "grads.hip"]
 HEADERS = ["ctm_common.h", "contract.h", "jacobi_internal.h", os.path.join("..", "..", "include", "ctm_hip.h")]
+# Python module that reads lists of tensors (host code only, against torch's own headers)
+EXT_SOURCE = os.path.join(HERE, "lists.cpp")
+EXT = os.path.join(PKG, "_ctm_lists.so")
 # no packed single-precision arithmetic (v_pk_*_f32): some of its forms have given wrong results on this hardware
 FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 LIB = os.path.join(PKG, "libctm_hip.so")
@@ -33,10 +36,27 @@ def asan_runtime():
     return os.path.realpath(subprocess.check_output(["gcc", "-print-file-name=libasan.so"], text=True).strip())
 
 
+def build_ext(force=False, verbose=True):
+    deps = [EXT_SOURCE, os.path.join(HERE, "..", "..", "include", "ctm_hip.h")]
+    if not force and os.path.exists(EXT) and all(os.path.getmtime(EXT) >= os.path.getmtime(d) for d in deps):
+        return EXT
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], EXT_SOURCE, "-o", EXT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return EXT
+
+
 def build(force=False, verbose=True, asan=False):
     srcs = [os.path.join(HERE, s) for s in SOURCES]
     deps = srcs + [os.path.join(HERE, h) for h in HEADERS]
     LIB = LIB_ASAN if asan else globals()["LIB"]
+    build_ext(force, verbose)
     if not force and os.path.exists(LIB) and all(os.path.getmtime(LIB) >= os.path.getmtime(d) for d in deps):
         return LIB
     objdir = os.path.join(HERE, "build_asan" if asan else "build")

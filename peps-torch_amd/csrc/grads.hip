@@ -12,41 +12,82 @@
 namespace {
 
 // Tensors of one launch: their table travels by value in the kernel arguments (no host-to-device copy, so a call may be captured).  64 = one
-// wave: the lookup "which tensor holds granule q" is one comparison per lane and a population count.
+// wave: the lookup "which tensor holds chunk q" is one comparison per lane and a population count.
 constexpr int TAB = 64;
-constexpr int GRANULE = 1024;          // doubles: unit in which the work of a launch is dealt out to its workgroups
 constexpr int THREADS = 256;
+constexpr int UNROLL = 4;              // 16-byte loads in flight per thread
+constexpr int CHUNK = 2 * THREADS * UNROLL;      // doubles: what a workgroup takes at a time; a chunk lies in one tensor
 constexpr int WS_HEAD = 4;             // ws: N2, Ninf, c, unused, then the partial results (4 doubles each)
 constexpr int PARTIALS = 1024;         // workgroups of the norm pass over all launches, up to one more per launch
 
 template <int NP> struct Table {
     double* p[NP][TAB];
     long long n[TAB];                  // doubles (a complex element counts two)
-    unsigned first[TAB + 1];           // granules before tensor t; entries behind the last tensor hold the total
+    unsigned first[TAB + 1];           // chunks before tensor t; entries behind the last tensor hold the total
 };
 
 typedef double d2 __attribute__((ext_vector_type(2)));
 typedef d2 d2u __attribute__((aligned(8)));          // 16-byte access at 8-byte alignment: views into a flat buffer start anywhere
 
-// tensor of granule q: the lanes of a wave compare one table entry each
-template <int NP> __device__ __forceinline__ int tensor_of(const Table<NP>& t, unsigned q) {
-    const int lane = threadIdx.x & 63;
-    return __popcll(__ballot(t.first[lane + 1] <= q));
+template <bool NT> __device__ __forceinline__ d2 load2(const double* x) {
+    if (NT) return __builtin_nontemporal_load((const d2u*)x);
+    return *(const d2u*)x;
+}
+template <bool NT> __device__ __forceinline__ void store2(double* x, d2 v) {
+    if (NT) __builtin_nontemporal_store((d2u)v, (d2u*)x);
+    else *(d2u*)x = v;
 }
 
-// Runs body(tensor, begin, end) over the segments (in doubles) of this workgroup's share of the granules.
-template <int NP, class F> __device__ __forceinline__ void segments(const Table<NP>& t, F&& body) {
-    const unsigned long long G = t.first[TAB];
-    unsigned q = (unsigned)(G * blockIdx.x / gridDim.x);
-    const unsigned qe = (unsigned)(G * (blockIdx.x + 1) / gridDim.x);
-    while (q < qe) {
-        const int k = __builtin_amdgcn_readfirstlane(tensor_of(t, q));
-        const unsigned f = t.first[k], l = t.first[k + 1];
-        const unsigned e = l < qe ? l : qe;
-        const long long n = t.n[k];
-        const long long a = (long long)(q - f) * GRANULE, b = (long long)(e - f) * GRANULE;
-        body(k, a, b < n ? b : n);
-        q = e;
+// Runs body(pointers, first double, length of the tensor) over this workgroup's chunks: every gridDim.x-th one, so that all workgroups sweep the
+// list together (measured on 545 MB: 87 us for the norm pass against 95 with one contiguous share per workgroup, 185 against 223 for the
+// scaling).  REVERSE: from the list's end to its beginning -- a second pass meets first what the pass before it left in the 256 MB last-level cache.
+template <int NP, bool REVERSE, class F> __device__ __forceinline__ void chunks(const Table<NP>& t, F&& body) {
+    const unsigned G = t.first[TAB], mine = t.first[(threadIdx.x & 63) + 1];
+    unsigned f = 0, l = 0;
+    long long n = 0;
+    double* p[NP] = {};
+    for (unsigned c = blockIdx.x; c < G; c += gridDim.x) {
+        const unsigned q = REVERSE ? G - 1 - c : c;
+        if (q < f || q >= l) {
+            const int k = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine <= q)));
+            f = t.first[k];
+            l = t.first[k + 1];
+            n = t.n[k];
+#pragma unroll
+            for (int j = 0; j < NP; ++j) p[j] = t.p[j][k];
+        }
+        body(p, (long long)(q - f) * CHUNK, n);
+    }
+}
+
+// Elements a + 2 u THREADS (+ 1) of this thread, zero behind the end of the tensor
+template <bool NT> __device__ __forceinline__ void load_chunk(d2 (&v)[UNROLL], const double* x, long long a, long long n) {
+    const long long i = a + 2 * threadIdx.x;
+    if (a + CHUNK <= n) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) v[u] = load2<NT>(x + i + u * 2 * THREADS);
+    } else {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const long long j = i + u * 2 * THREADS;
+            v[u] = d2{0.0, 0.0};
+            if (j + 1 < n) v[u] = load2<NT>(x + j);
+            else if (j < n) v[u].x = x[j];               // (real tensors of odd length)
+        }
+    }
+}
+template <bool NT> __device__ __forceinline__ void store_chunk(const d2 (&v)[UNROLL], double* x, long long a, long long n) {
+    const long long i = a + 2 * threadIdx.x;
+    if (a + CHUNK <= n) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) store2<NT>(x + i + u * 2 * THREADS, v[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const long long j = i + u * 2 * THREADS;
+            if (j + 1 < n) store2<NT>(x + j, v[u]);
+            else if (j < n) x[j] = v[u].x;
+        }
     }
 }
 
@@ -93,23 +134,24 @@ __device__ __forceinline__ double wave_sum(double x) {
     return x;
 }
 
-// Partial result of a workgroup of `WAVES` waves, valid on thread 0.
+__device__ __forceinline__ void join(Part& p, const Part& q) {
+    p.big += q.big; p.med += q.med; p.small += q.small; p.top = umax(p.top, q.top);
+}
+
+// Result of a workgroup of `WAVES` waves, the same bits on all its threads.
 template <int WAVES> __device__ __forceinline__ Part reduce_block(Part p) {
     __shared__ Part sh[WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     p.med = wave_sum(p.med);
     if (__any(p.big != 0.0)) p.big = wave_sum(p.big);          // (true for NaN)
     if (__any(p.small != 0.0)) p.small = wave_sum(p.small);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) p.top = umax(p.top, __shfl_xor(p.top, o));
-    if (WAVES == 1) return p;
-    if (lane == 0) sh[wave] = p;
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = p;
     __syncthreads();
-    if (threadIdx.x == 0)
-        for (int w = 1; w < WAVES; ++w) {
-            p.big += sh[w].big; p.med += sh[w].med; p.small += sh[w].small; p.top = umax(p.top, sh[w].top);
-        }
-    return p;
+    Part r = sh[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) join(r, sh[w]);
+    return r;
 }
 
 template <bool CPLX> __device__ __forceinline__ Part part_of(const Acc& a) {
@@ -121,86 +163,149 @@ template <bool CPLX> __device__ __forceinline__ Part part_of(const Acc& a) {
 struct Bound { double max_norm; int inf_norm; };      // max_norm < 0: no bound
 
 // N2, Ninf and the factor c from the three range sums
-__device__ __forceinline__ void finish(const Part& p, Bound bd, double* ws) {
-    double n2;
-    if (p.big != 0.0) n2 = sqrt(fma(p.med * 0x1p-600, 0x1p-600, p.big)) * 0x1p600;
-    else if (p.med != 0.0) n2 = sqrt(fma(p.small * 0x1p-600, 0x1p-600, p.med));
-    else n2 = sqrt(p.small) * 0x1p-600;
-    const double ninf = __longlong_as_double((long long)p.top);
-    const double n = bd.inf_norm ? ninf : n2;
-    ws[0] = n2;
-    ws[1] = ninf;
-    ws[2] = (bd.max_norm < 0.0 || n <= bd.max_norm) ? 1.0 : bd.max_norm / n;      // NaN norm: NaN
+struct Norms { double n2, ninf, c; };
+__device__ __forceinline__ Norms finish(const Part& p, Bound bd) {
+    Norms r;
+    if (p.big != 0.0) r.n2 = sqrt(fma(p.med * 0x1p-600, 0x1p-600, p.big)) * 0x1p600;
+    else if (p.med != 0.0) r.n2 = sqrt(fma(p.small * 0x1p-600, 0x1p-600, p.med));
+    else r.n2 = sqrt(p.small) * 0x1p-600;
+    r.ninf = __longlong_as_double((long long)p.top);
+    const double n = bd.inf_norm ? r.ninf : r.n2;
+    r.c = (bd.max_norm < 0.0 || n <= bd.max_norm) ? 1.0 : bd.max_norm / n;      // NaN norm: NaN
+    return r;
 }
+__device__ __forceinline__ void put_norms(const Norms& r, double* ws) { ws[0] = r.n2; ws[1] = r.ninf; ws[2] = r.c; }
 
-template <bool CPLX>
+// First pass: partial results of the workgroups.
+template <bool CPLX, bool NT>
 __global__ __launch_bounds__(THREADS) void norm_partials_kernel(const Table<1> t, Part* out) {
     Acc acc;
-    segments(t, [&](int k, long long a, long long b) {
-        const double* x = t.p[0][k];
-        long long i = a + 2 * threadIdx.x;
-        for (; i + 3 * 2 * THREADS + 1 < b; i += 4 * 2 * THREADS) {
-            d2 v[4];
+    chunks<1, false>(t, [&](double* const (&p)[1], long long a, long long n) {
+        d2 v[UNROLL];
+        load_chunk<NT>(v, p[0], a, n);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = *(const d2u*)(x + i + u * 2 * THREADS);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) add<CPLX>(acc, v[u]);
-        }
-        for (; i + 1 < b; i += 2 * THREADS) add<CPLX>(acc, *(const d2u*)(x + i));
-        if (i < b) { d2 v = {x[i], 0.0}; add<CPLX>(acc, v); }          // (real tensors of odd length)
+        for (int u = 0; u < UNROLL; ++u) add<CPLX>(acc, v[u]);
     });
     const Part p = reduce_block<THREADS / 64>(part_of<CPLX>(acc));
     if (threadIdx.x == 0) out[blockIdx.x] = p;
 }
 
-__global__ __launch_bounds__(1024) void norm_finish_kernel(const Part* part, int np, Bound bd, double* ws) {
+// Norms from the partial results, by a workgroup of T threads, in an order that depends on T and np alone
+template <int T> __device__ __forceinline__ Norms join_partials(const Part* part, int np, Bound bd) {
     Part p{0.0, 0.0, 0.0, 0};
-    for (int i = threadIdx.x; i < np; i += 1024) {
-        const Part q = part[i];
-        p.big += q.big; p.med += q.med; p.small += q.small; p.top = umax(p.top, q.top);
-    }
-    p = reduce_block<16>(p);
-    if (threadIdx.x == 0) finish(p, bd, ws);
+    for (int i = threadIdx.x; i < np; i += T) join(p, part[i]);
+    return finish(reduce_block<T / 64>(p), bd);
+}
+
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const Part* part, int np, Bound bd, double* ws) {
+    const Norms r = join_partials<1024>(part, np, bd);
+    if (threadIdx.x == 0) put_norms(r, ws);
+}
+
+// Where the second pass gets its factor from: every workgroup joins the partial results by itself (32 kB at most, from the L2 cache; all get the
+// same bits), which is cheaper than a kernel in between.
+struct Source { const Part* part; int np; Bound bd; double* ws; };      // ws: the norms are written there (by one workgroup); may be null
+__device__ __forceinline__ double factor(const Source& s) {
+    if (s.bd.max_norm < 0.0) return 1.0;
+    const Norms r = join_partials<THREADS>(s.part, s.np, s.bd);
+    if (s.ws && blockIdx.x == 0 && threadIdx.x == 0) put_norms(r, s.ws);
+    return r.c;
 }
 
 // y = c x (p[0] = x, p[1] = y).  A list inside the bound (c = 1) is left untouched in place.
-__global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const double* ws) {
-    const double c = ws[2];
-    segments(t, [&](int k, long long a, long long b) {
-        const double* x = t.p[0][k];
-        double* y = t.p[1][k];
-        if (c == 1.0 && x == y) return;
-        for (long long i = a + 2 * threadIdx.x; i < b; i += 2 * THREADS) {
-            if (i + 1 < b) { const d2 v = *(const d2u*)(x + i); *(d2u*)(y + i) = v * c; }
-            else y[i] = x[i] * c;
-        }
+template <bool NT>
+__global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const Source s) {
+    const double c = factor(s);
+    chunks<2, true>(t, [&](double* const (&p)[2], long long a, long long n) {
+        if (c == 1.0 && p[0] == p[1]) return;
+        d2 v[UNROLL];
+        load_chunk<false>(v, p[0], a, n);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) v[u] *= c;
+        store_chunk<NT>(v, p[1], a, n);
     });
 }
 
-struct Step { double lr, mu, one_minus_tau; int first, bounded; };
+struct Step { double lr, mu, one_minus_tau; int first; };
+
+// d = c g -> the new momentum (MOMENTUM), p -> the new parameters
+template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d, d2 m, double c, const Step& s) {
+    d *= c;
+    if (MOMENTUM && !s.first) d = m * s.mu + d * s.one_minus_tau;
+    p -= d * s.lr;
+}
 
 // p[0] = parameters, p[1] = gradients, p[2] = momentum buffers (MOMENTUM)
-template <bool MOMENTUM, class V> __device__ __forceinline__ void step_one(double* p, const double* g, double* m, long long i, double c, const Step& s) {
-    V d = *(const V*)(g + i) * c;
-    if (MOMENTUM) {
-        if (!s.first) d = *(const V*)(m + i) * s.mu + d * s.one_minus_tau;
-        *(V*)(m + i) = d;
-    }
-    *(V*)(p + i) = *(const V*)(p + i) - d * s.lr;
+template <bool MOMENTUM, bool NT>
+__global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 : 2> t, const Step s, const Source src) {
+    const double c = factor(src);
+    chunks<MOMENTUM ? 3 : 2, true>(t, [&](double* const (&p)[MOMENTUM ? 3 : 2], long long a, long long n) {
+        d2 x[UNROLL], d[UNROLL], m[UNROLL];
+        load_chunk<false>(d, p[1], a, n);
+        if (MOMENTUM && !s.first) load_chunk<false>(m, p[MOMENTUM ? 2 : 0], a, n);
+        load_chunk<false>(x, p[0], a, n);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) step_pair<MOMENTUM>(x[u], d[u], m[u], c, s);
+        if (MOMENTUM) store_chunk<NT>(d, p[MOMENTUM ? 2 : 0], a, n);
+        store_chunk<NT>(x, p[0], a, n);
+    });
 }
 
-template <bool MOMENTUM>
-__global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 : 2> t, Step s, const double* ws) {
-    const double c = s.bounded ? ws[2] : 1.0;
-    segments(t, [&](int k, long long a, long long b) {
-        double* p = t.p[0][k];
-        const double* g = t.p[1][k];
-        double* m = MOMENTUM ? t.p[MOMENTUM ? 2 : 0][k] : nullptr;
-        for (long long i = a + 2 * threadIdx.x; i < b; i += 2 * THREADS) {
-            if (i + 1 < b) step_one<MOMENTUM, d2u>(p, g, m, i, c, s);
-            else step_one<MOMENTUM, double>(p, g, m, i, c, s);
+// Short lists: one workgroup, one launch, the list in registers between the norm and the second use.  Its 16 waves take pieces of 128 doubles.
+constexpr int PIECE = 128, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
+enum { OP_NORMS, OP_CLIP, OP_SGD, OP_SGD_MOMENTUM };
+template <int OP> struct Shape { static constexpr int NP = OP == OP_NORMS ? 1 : OP == OP_SGD_MOMENTUM ? 3 : 2, READ = OP >= OP_SGD ? 1 : 0, ROUNDS = OP >= OP_SGD ? 4 : 8; };
+
+__device__ __forceinline__ d2 load_piece(const double* x, int i, int n) {
+    d2 v = {0.0, 0.0};
+    if (i + 1 < n) v = load2<false>(x + i);
+    else if (i < n) v.x = x[i];
+    return v;
+}
+__device__ __forceinline__ void store_piece(d2 v, double* x, int i, int n) {
+    if (i + 1 < n) store2<false>(x + i, v);
+    else if (i < n) x[i] = v.x;
+}
+
+template <int OP, bool CPLX>
+__global__ __launch_bounds__(SMALL_THREADS) void small_kernel(const Table<Shape<OP>::NP> t, const Bound bd, const Step s, double* ws) {
+    using S = Shape<OP>;
+    const unsigned G = t.first[TAB], lane = threadIdx.x & 63, mine = t.first[lane + 1];
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int k[S::ROUNDS], i[S::ROUNDS], n[S::ROUNDS];
+    d2 v[S::ROUNDS], x[S::ROUNDS], m[S::ROUNDS];
+#pragma unroll
+    for (int r = 0; r < S::ROUNDS; ++r) {
+        const unsigned q = wave + r * SMALL_WAVES;
+        v[r] = d2{0.0, 0.0};
+        if (q < G) {
+            k[r] = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine <= q)));
+            i[r] = (int)(q - t.first[k[r]]) * PIECE + 2 * (int)lane;
+            n[r] = (int)t.n[k[r]];
+            v[r] = load_piece(t.p[S::READ][k[r]], i[r], n[r]);
+            if (OP >= OP_SGD) x[r] = load_piece(t.p[0][k[r]], i[r], n[r]);
+            if (OP == OP_SGD_MOMENTUM) m[r] = load_piece(t.p[S::NP - 1][k[r]], i[r], n[r]);
         }
-    });
+    }
+    Acc acc;
+#pragma unroll
+    for (int r = 0; r < S::ROUNDS; ++r)
+        if (wave + r * SMALL_WAVES < G) add<CPLX>(acc, v[r]);
+    const Norms nr = finish(reduce_block<SMALL_WAVES>(part_of<CPLX>(acc)), bd);
+    if (threadIdx.x == 0) put_norms(nr, ws);
+    if (OP == OP_NORMS) return;
+#pragma unroll
+    for (int r = 0; r < S::ROUNDS; ++r) {
+        if (wave + r * SMALL_WAVES >= G) return;
+        if (OP == OP_CLIP) {
+            double* y = t.p[S::NP - 1][k[r]];
+            if (nr.c != 1.0 || y != t.p[0][k[r]]) store_piece(v[r] * nr.c, y, i[r], n[r]);
+        } else {
+            step_pair<OP == OP_SGD_MOMENTUM>(x[r], v[r], m[r], nr.c, s);
+            if (OP == OP_SGD_MOMENTUM) store_piece(v[r], t.p[S::NP - 1][k[r]], i[r], n[r]);
+            store_piece(x[r], t.p[0][k[r]], i[r], n[r]);
+        }
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
@@ -263,7 +368,7 @@ template <int NP> int check_lists(ctm_ctx* ctx, const char* name, const Lists<NP
 }
 
 // The next launch's table from tensor `i` on; returns the index behind its last tensor.
-template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t) {
+template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t, int chunk = CHUNK) {
     int k = 0;
     unsigned q = 0;
     for (; i < L.nt && k < TAB; ++i) {
@@ -271,7 +376,7 @@ template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t) {
         for (int j = 0; j < NP; ++j) t.p[j][k] = const_cast<double*>(L.p[j][i]);
         t.n[k] = L.n[i] * L.unit;
         t.first[k++] = q;
-        q += (unsigned)((t.n[k - 1] + GRANULE - 1) / GRANULE);
+        q += (unsigned)((t.n[k - 1] + chunk - 1) / chunk);
     }
     for (int j = k; j <= TAB; ++j) t.first[j] = q;
     return i;
@@ -290,33 +395,71 @@ template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t) {
         }                                                                                                         \
     } while (0)
 
-unsigned granules_of(const long long* n, int nt, long long unit) {
-    unsigned long long g = 0;
-    for (int i = 0; i < nt; ++i) g += (unsigned long long)((n[i] * unit + GRANULE - 1) / GRANULE);
-    return (unsigned)g;
+// What the choice of a kernel goes by: chunks and bytes of the list, whether one workgroup takes all of it
+struct Size { unsigned chunks; int tensors; long long pieces, bytes; };
+Size size_of(const long long* n, int nt, long long unit) {
+    Size s{0, 0, 0, 0};
+    for (int i = 0; i < nt; ++i) {
+        const long long d = n[i] * unit;
+        s.chunks += (unsigned)((d + CHUNK - 1) / CHUNK);
+        s.pieces += (d + PIECE - 1) / PIECE;
+        s.tensors += d > 0;
+        s.bytes += 8 * d;
+    }
+    return s;
 }
+bool is_small(const Size& z, int rounds) { return z.tensors <= TAB && z.pieces <= rounds * SMALL_WAVES; }
 
-int norms(ctm_ctx* ctx, hipStream_t s, int nt, const double* const* x, const long long* n, Bound bd, double* ws) {
-    Lists<1> L{nt, {x}, n, ctx->cplx ? 2 : 1};
-    const unsigned long long total = granules_of(n, nt, L.unit);
+// Lists that do not fit the 256 MB last-level cache are read once without a claim on it (545 MB: 82 us against 87); stores of lists longer than
+// the 32 MB of L2 cache bypass it (545 MB scaled in 185 us against 188 ... 229, 1.1 GB after its norm pass in 556 against 591).
+constexpr long long LLC_BYTES = 256LL << 20, L2_BYTES = 32LL << 20;
+
+template <bool NT> int partials(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, double* ws, int* np) {
+    *np = 0;
     Part* part = (Part*)(ws + WS_HEAD);
-    int np = 0;
-    for (int i = 0; i < nt;) {
+    for (int i = 0; i < L.nt;) {
         Table<1> t;
         i = fill(L, i, t);
         const unsigned long long g = t.first[TAB];
         if (!g) break;
-        unsigned long long grid = PARTIALS * g / total;
-        grid = grid < 1 ? 1 : grid > g ? g : grid;
-        if (ctx->cplx) GRADS_LAUNCH(ctx, s, norm_partials_kernel<true>, (unsigned)grid, THREADS, t, part + np);
-        else GRADS_LAUNCH(ctx, s, norm_partials_kernel<false>, (unsigned)grid, THREADS, t, part + np);
-        np += (int)grid;
+        unsigned long long grid = z.chunks <= PARTIALS ? g : PARTIALS * g / z.chunks;
+        if (grid < 1) grid = 1;
+        if (ctx->cplx) GRADS_LAUNCH(ctx, s, (norm_partials_kernel<true, NT>), (unsigned)grid, THREADS, t, part + *np);
+        else GRADS_LAUNCH(ctx, s, (norm_partials_kernel<false, NT>), (unsigned)grid, THREADS, t, part + *np);
+        *np += (int)grid;
     }
-    GRADS_LAUNCH(ctx, s, norm_finish_kernel, 1, 1024, (const Part*)part, np, bd, ws);
     return CTM_OK;
 }
 
-constexpr unsigned MAX_GRID = 4096;
+template <int OP> int small(ctm_ctx* ctx, hipStream_t s, const Lists<Shape<OP>::NP>& L, Bound bd, const Step& st, double* ws) {
+    Table<Shape<OP>::NP> t;
+    fill(L, 0, t, PIECE);
+    if (ctx->cplx) GRADS_LAUNCH(ctx, s, (small_kernel<OP, true>), 1, SMALL_THREADS, t, bd, st, ws);
+    else GRADS_LAUNCH(ctx, s, (small_kernel<OP, false>), 1, SMALL_THREADS, t, bd, st, ws);
+    return CTM_OK;
+}
+
+// Second pass over a list: launch(table, grid, source) for every table of it.
+constexpr unsigned MAX_GRID = 8192;
+template <int NP, class F> int second_pass(const Lists<NP>& L, Source src, F&& launch) {
+    for (int i = 0; i < L.nt;) {
+        Table<NP> t;
+        i = fill(L, i, t);
+        const unsigned g = t.first[TAB];
+        if (!g) break;
+        CTM_TRY(launch(t, g < MAX_GRID ? g : MAX_GRID, src));
+        src.ws = nullptr;                    // the norms are written once
+    }
+    return CTM_OK;
+}
+
+template <bool MOMENTUM> int sgd(ctm_ctx* ctx, hipStream_t s, const Lists<MOMENTUM ? 3 : 2>& L, const Size& z, const Step& st, const Source& src) {
+    return second_pass(L, src, [&](const Table<MOMENTUM ? 3 : 2>& t, unsigned grid, const Source& f) -> int {
+        if (z.bytes > L2_BYTES) GRADS_LAUNCH(ctx, s, (sgd_kernel<MOMENTUM, true>), grid, THREADS, t, st, f);
+        else GRADS_LAUNCH(ctx, s, (sgd_kernel<MOMENTUM, false>), grid, THREADS, t, st, f);
+        return CTM_OK;
+    });
+}
 
 }  // namespace
 
@@ -328,7 +471,16 @@ int ctm_grad_norms(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* 
     const bool written[1] = {false};
     CTM_TRY(check_lists<1>(ctx, "grad_norms", Lists<1>{nt, {x}, n, ctx->cplx ? 2 : 1}, written, 0));
     if (!ws || ws_doubles < CTM_GRAD_WS_DOUBLES((long long)nt)) return list_error(ctx, "grad_norms", "workspace too small (CTM_GRAD_WS_DOUBLES)");
-    return norms(ctx, (hipStream_t)hip_stream, nt, x, n, Bound{-1.0, 0}, ws);
+    hipStream_t s = (hipStream_t)hip_stream;
+    const Lists<1> L{nt, {x}, n, ctx->cplx ? 2 : 1};
+    const Size z = size_of(n, nt, L.unit);
+    const Bound none{-1.0, 0};
+    if (is_small(z, Shape<OP_NORMS>::ROUNDS)) return small<OP_NORMS>(ctx, s, L, none, Step{}, ws);
+    int np;
+    if (z.bytes > LLC_BYTES) CTM_TRY(partials<true>(ctx, s, L, z, ws, &np));
+    else CTM_TRY(partials<false>(ctx, s, L, z, ws, &np));
+    GRADS_LAUNCH(ctx, s, norm_finish_kernel, 1, 1024, (const Part*)(ws + WS_HEAD), np, none, ws);
+    return CTM_OK;
     });
 }
 
@@ -343,15 +495,16 @@ int ctm_grad_clip(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x
     if (norm_type != CTM_NORM_2 && norm_type != CTM_NORM_INF) return list_error(ctx, "grad_clip", "norm_type must be CTM_NORM_2 or CTM_NORM_INF");
     if (!ws || ws_doubles < CTM_GRAD_WS_DOUBLES((long long)nt)) return list_error(ctx, "grad_clip", "workspace too small (CTM_GRAD_WS_DOUBLES)");
     hipStream_t s = (hipStream_t)hip_stream;
-    CTM_TRY(norms(ctx, s, nt, x, n, Bound{max_norm, norm_type == CTM_NORM_INF}, ws));
-    for (int i = 0; i < nt;) {
-        Table<2> t;
-        i = fill(L, i, t);
-        const unsigned g = t.first[TAB];
-        if (!g) break;
-        GRADS_LAUNCH(ctx, s, clip_kernel, g < MAX_GRID ? g : MAX_GRID, THREADS, t, (const double*)ws);
-    }
-    return CTM_OK;
+    const Bound bd{max_norm, norm_type == CTM_NORM_INF};
+    const Size z = size_of(n, nt, L.unit);
+    if (is_small(z, Shape<OP_CLIP>::ROUNDS)) return small<OP_CLIP>(ctx, s, L, bd, Step{}, ws);
+    int np;
+    CTM_TRY(partials<false>(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, ws, &np));
+    return second_pass(L, Source{(const Part*)(ws + WS_HEAD), np, bd, ws}, [&](const Table<2>& t, unsigned grid, const Source& f) -> int {
+        if (z.bytes > L2_BYTES) GRADS_LAUNCH(ctx, s, clip_kernel<true>, grid, THREADS, t, f);
+        else GRADS_LAUNCH(ctx, s, clip_kernel<false>, grid, THREADS, t, f);
+        return CTM_OK;
+    });
     });
 }
 
@@ -370,24 +523,16 @@ int ctm_sgd_step(ctm_ctx* ctx, void* hip_stream, int nt, double* const* p, const
     if (bounded) {
         if (norm_type != CTM_NORM_2 && norm_type != CTM_NORM_INF) return list_error(ctx, "sgd_step", "norm_type must be CTM_NORM_2 or CTM_NORM_INF");
         if (!ws || ws_doubles < CTM_GRAD_WS_DOUBLES((long long)nt)) return list_error(ctx, "sgd_step", "workspace too small (CTM_GRAD_WS_DOUBLES)");
-        CTM_TRY(norms(ctx, s, nt, g, n, Bound{max_norm, norm_type == CTM_NORM_INF}, ws));
     }
-    const Step st{lr, momentum, 1.0 - dampening, first, bounded};
-    for (int i = 0; i < nt;) {
-        unsigned q;
-        if (m) {
-            Table<3> t;
-            i = fill(L3, i, t);
-            if (!(q = t.first[TAB])) break;
-            GRADS_LAUNCH(ctx, s, sgd_kernel<true>, q < MAX_GRID ? q : MAX_GRID, THREADS, t, st, (const double*)ws);
-        } else {
-            Table<2> t;
-            i = fill(L2, i, t);
-            if (!(q = t.first[TAB])) break;
-            GRADS_LAUNCH(ctx, s, sgd_kernel<false>, q < MAX_GRID ? q : MAX_GRID, THREADS, t, st, (const double*)ws);
-        }
+    const Step st{lr, momentum, 1.0 - dampening, first};
+    const Size z = size_of(n, nt, L2.unit);
+    Source src{nullptr, 0, Bound{bounded ? max_norm : -1.0, norm_type == CTM_NORM_INF}, ws};
+    if (bounded) {
+        if (is_small(z, Shape<OP_SGD>::ROUNDS)) return m ? small<OP_SGD_MOMENTUM>(ctx, s, L3, src.bd, st, ws) : small<OP_SGD>(ctx, s, L2, src.bd, st, ws);
+        CTM_TRY(partials<false>(ctx, s, Lists<1>{nt, {g}, n, L2.unit}, z, ws, &src.np));
+        src.part = (const Part*)(ws + WS_HEAD);
     }
-    return CTM_OK;
+    return m ? sgd<true>(ctx, s, L3, z, st, src) : sgd<false>(ctx, s, L2, z, st, src);
     });
 }
 

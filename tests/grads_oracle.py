@@ -26,10 +26,10 @@ def norms(arrays):
 
 def tol_n2(n):
     """Relative bound on the 2-norm of n doubles.  Every square sum is of non-negative terms, so each addition or fused product costs a relative U
-    of the result at most: per thread the pairs of its share (n / (2 * 256) over at most 1024 workgroups, never more than 4 loads of a short
-    share and one per granule's end of each of <= 512 tensors it meets), 2 roundings of a pair's own squares, 6 levels of the wave, 3 of the
-    workgroup, up to 4 + 6 + 16 of the last combination; half of it through the root, one rounding of the root, one of the input's scaling."""
-    depth = n / (2.0 * 256 * 1024) + 64 + 2 + 6 + 3 + 26
+    of the result at most: per thread the pairs of its chunks (n / (2 * 256) over at most 1024 workgroups, and up to 4 more for the short chunk
+    at the end of each of the tensors it meets, fewer than 16 here), 2 roundings of a pair's own squares, 6 levels of the wave, up to 16 of the
+    workgroup, 5 + 6 + 3 of the last combination; half of it through the root, one rounding of the root, one of the scaling by a power of two."""
+    depth = n / (2.0 * 256 * 1024) + 64 + 2 + 6 + 16 + 14
     return (depth / 2 + 2) * U
 
 

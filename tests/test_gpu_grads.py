@@ -72,8 +72,10 @@ def check_step(p1, m1, p0, m0, g, c, ctol, lr, mu, tau, first):
 
 
 LISTS = {
-    "one": [1], "empty_tensor": [0], "two": [2], "odd": [7], "granule": [1023, 1024, 1025], "granules": [2047, 2048, 2049, 4097],
-    "empties_between": [0, 5, 0, 0, 513, 0], "single_block_edge": [16383, 1], "over_edge": [16385], "cell_D4": [512] * 4, "cell_D8": [8192] * 8,
+    "one": [1], "empty_tensor": [0], "two": [2], "odd": [7], "loads": [511, 512, 513, 1023, 1024, 1025], "chunk": [2047, 2048, 2049],
+    "chunks": [4095, 4096, 8191, 8193],
+    "empties_between": [0, 5, 0, 0, 513, 0], "pieces": [127, 128, 129, 255], "one_group": [16384], "one_group_half": [8192], "one_group_quarter": [4096],
+    "group_of_many": [256] * 63 + [255], "group_and_one": [16383, 1], "over_group": [16385], "cell_D4": [512] * 4, "cell_D8": [8192] * 8,
     "table_full": [3] * 64, "table_over": [5] * 65, "many": [(37 * i) % 411 for i in range(300)], "long": [1 << 20, 3, 777777],
     "one_long": [5000001],
 }

@@ -6,6 +6,7 @@ import json
 import logging
 import math
 import os
+import threading
 import numpy as np
 import pytest
 import torch
@@ -67,20 +68,38 @@ class HostLib:
 
 
 class HostEngine(_native.Engine):
-    def __init__(self):
-        self.lib, self.device = HostLib(), torch.device("cpu")
+    """`short`: with the module that reads plain lists (csrc/lists.cpp), its entries the double's."""
+
+    def __init__(self, short=False):
+        self.lib, self.device, self._handles = HostLib(), torch.device("cpu"), {}
+        if short:
+            self._lists, self._short_calls = _native.load_lists(), 0
+            self._handles = {torch.float64: C.c_void_p(8), torch.complex128: C.c_void_p(16)}
+            self._keep = {}
+            for n in ("grad_norms", "grad_clip", "sgd_step"):
+                sig = _native._SIGS["ctm_" + n]
+
+                def entry(h, *a, n=n):
+                    self.lib.cplx = h == 16
+                    self._short_calls += 1
+                    return getattr(self.lib, "ctm_" + n)(h, *[v if v or not isinstance(v, C._Pointer) else None for v in a])
+                self._keep[n] = C.CFUNCTYPE(C.c_int, *sig)(entry)
+            self._entries = {n: C.cast(f, C.c_void_p).value for n, f in self._keep.items()}
 
     def __del__(self):
         pass
+
+    def _stream(self):
+        return 0
 
     def _run_lists(self, what, dt, fn):
         self.lib.cplx = dt.is_complex
         self._ck(fn(None, None), what)
 
 
-@pytest.fixture
-def host():
-    e = HostEngine()
+@pytest.fixture(params=[False, True], ids=["general", "short"])
+def host(request):
+    e = HostEngine(request.param)
     backend.set_engine(e)
     yield e
     backend.set_engine(None)
@@ -154,6 +173,43 @@ def test_refusals_before_anything_is_written(host):
             call()
     assert not host.lib.calls
     assert torch.equal(t, torch.ones_like(t)) and torch.equal(u, torch.ones_like(u))
+
+
+def test_which_lists_go_the_short_way():
+    """Contiguous tensors of one dtype, in any number; the rest goes the general way with the same results."""
+    e, d = HostEngine(True), HostEngine()
+    for dt in (torch.float64, torch.complex128):
+        ts = [t64(n, dtype=dt, seed=n) for n in (1, 0, 7, 300)]
+        assert torch.equal(e.grad_norms(ts), d.grad_norms(ts)) and torch.equal(e.grad_norms(tuple(ts)), d.grad_norms(iter(ts)))
+        a, b = [t.clone() for t in ts], [t.clone() for t in ts]
+        v = a[2]._version
+        assert torch.equal(e.clip_grads(a, 0.5), d.clip_grads(b, 0.5)) and a[2]._version == v + 1
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+        o = [torch.zeros_like(t) for t in ts]
+        e.clip_grads(ts, 0.5, INF, out=o)
+        d.clip_grads(ts, 0.5, INF, out=b)
+        assert all(torch.equal(x, y) for x, y in zip(o, b)) and o[2]._version > 0
+        p, q, m, k = ([t.clone() for t in ts] for _ in range(4))
+        got, want = (f.sgd_step(x, ts, y, lr=0.5, momentum=0.5, dampening=0.25, first=0, max_norm=0.5) for f, x, y in ((e, p, m), (d, q, k)))
+        assert torch.equal(got, want) and all(torch.equal(x, y) for x, y in zip(p + m, q + k))
+        assert e.sgd_step(p, ts, lr=0.5) is None and d.sgd_step(q, ts, lr=0.5) is None and all(torch.equal(x, y) for x, y in zip(p, q))
+        calls = e._short_calls
+        odd = [t64(4, 3, dtype=dt).t()]
+        assert torch.equal(e.grad_norms(odd), d.grad_norms(odd)) and torch.equal(e.grad_norms([]), d.grad_norms([])) and e._short_calls == calls
+    assert e._short_calls == 12
+    with torch.inference_mode():
+        x = torch.ones(3, dtype=torch.float64)
+        e.clip_grads([x], 0.0)
+        d.clip_grads([x], 0.0)
+    # a status of the library reaches the caller as its error
+    e._bind_dtype = lambda dt: None
+    e.lib.ctm_last_error = lambda h: b"in use"
+    busy = C.CFUNCTYPE(C.c_int, *_native._SIGS["ctm_grad_norms"])(lambda *a: 7)
+    e._entries["grad_norms"] = C.cast(busy, C.c_void_p).value
+    e._tls = threading.local()
+    e._tls.h = None
+    with pytest.raises(NativeError, match="busy"):
+        e.grad_norms([torch.ones(3, dtype=torch.float64)])
 
 
 def test_the_workspace_is_what_the_header_asks_for():
