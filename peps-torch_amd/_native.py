@@ -1112,6 +1112,7 @@ class Engine:
 
 
 _engines = {}
+_engine_of_name = {}        # device strings with an index ("cuda:0") -> engine
 
 
 def _shutdown():
@@ -1127,6 +1128,7 @@ def _shutdown():
         except Exception:
             pass
     _engines.clear()
+    _engine_of_name.clear()
 
 
 import atexit
@@ -1135,6 +1137,8 @@ atexit.register(_shutdown)
 
 def engine(device=None):
     """Process-wide engine per device (created lazily)."""
+    if type(device) is str and device in _engine_of_name:
+        return _engine_of_name[device]
     if not torch.cuda.is_available():
         raise NativeError("no HIP device visible: the CTM engine runs only on the GPU (no CPU fallback)")
     if device is None:
@@ -1150,4 +1154,6 @@ def engine(device=None):
         for kv in filter(None, os.environ.get("CTM_ENGINE_OPTS", "").split(",")):
             k, v = kv.split("=")
             _engines[idx].set_option(k.strip(), float(v))
+    if type(device) is str and d.index is not None:
+        _engine_of_name[device] = _engines[idx]
     return _engines[idx]

@@ -11,20 +11,23 @@
 
 namespace {
 
-// Tensors of one launch: their table travels by value in the kernel arguments (no host-to-device copy, so a call may be captured).  64 = one
-// wave: the lookup "which tensor holds chunk q" is one comparison per lane and a population count.
-constexpr int TAB = 64;
 constexpr int THREADS = 256;
 constexpr int UNROLL = 4;              // 16-byte loads in flight per thread
 constexpr int CHUNK = 2 * THREADS * UNROLL;      // doubles: what a workgroup takes at a time; a chunk lies in one tensor
 constexpr int WS_HEAD = 4;             // ws: N2, Ninf, c, unused, then the partial results (4 doubles each)
 constexpr int PARTIALS = 1024;         // workgroups of the norm pass over all launches, up to one more per launch
 
+// The tensors of one launch.  Their table travels by value in the kernel arguments (no host-to-device copy, so a call may be captured), which hold
+// 4 kB: addresses are 32-bit counts of doubles above the lowest one (tensors of a launch lie within 32 GB), lengths what the last chunk holds.
+// More tensors per launch, fewer launches -- each costs >= 4 us, more than the work on a hundred short tensors.
 template <int NP> struct Table {
-    double* p[NP][TAB];
-    long long n[TAB];                  // doubles (a complex element counts two)
-    unsigned first[TAB + 1];           // chunks before tensor t; entries behind the last tensor hold the total
+    static constexpr int N = NP == 1 ? 384 : NP == 2 ? 256 : 192;
+    double* base[NP];
+    unsigned offset[NP][N];
+    unsigned first[N + 1];             // chunks before tensor t; entries behind the last tensor hold the total
+    unsigned short tail[N];            // doubles of the last chunk, less one (a complex element counts two)
 };
+static_assert(sizeof(Table<1>) <= 3968 && sizeof(Table<2>) <= 3968 && sizeof(Table<3>) <= 3968, "the kernel arguments hold 4 kB");
 
 typedef double d2 __attribute__((ext_vector_type(2)));
 typedef d2 d2u __attribute__((aligned(8)));          // 16-byte access at 8-byte alignment: views into a flat buffer start anywhere
@@ -38,25 +41,43 @@ template <bool NT> __device__ __forceinline__ void store2(double* x, d2 v) {
     else *(d2u*)x = v;
 }
 
+// The tensor that holds chunk q: each lane of a wave compares N / 64 table entries, the count of those at or below q is its number.  The tensor
+// found last is tried first: chunks of long tensors need no lookup.
+template <int NP> struct Finder {
+    static constexpr int R = Table<NP>::N / 64;
+    const Table<NP>& t;
+    unsigned mine[R];
+    unsigned f = 0, l = 0;             // chunks of the tensor: f ... l - 1
+    long long n = 0;                   // its doubles
+    double* p[NP] = {};
+    __device__ __forceinline__ explicit Finder(const Table<NP>& table) : t(table) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) mine[j] = t.first[64 * j + (threadIdx.x & 63) + 1];
+    }
+    __device__ __forceinline__ void find(unsigned q, int chunk) {
+        if (q >= f && q < l) return;
+        int k = 0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) k += __popcll(__ballot(mine[j] <= q));
+        k = __builtin_amdgcn_readfirstlane(k);
+        f = t.first[k];
+        l = t.first[k + 1];
+        n = (long long)(l - f - 1) * chunk + t.tail[k] + 1;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) p[j] = t.base[j] + t.offset[j][k];
+    }
+};
+
 // Runs body(pointers, first double, length of the tensor) over this workgroup's chunks: every gridDim.x-th one, so that all workgroups sweep the
 // list together (measured on 545 MB: 87 us for the norm pass against 95 with one contiguous share per workgroup, 185 against 223 for the
 // scaling).  REVERSE: from the list's end to its beginning -- a second pass meets first what the pass before it left in the 256 MB last-level cache.
 template <int NP, bool REVERSE, class F> __device__ __forceinline__ void chunks(const Table<NP>& t, F&& body) {
-    const unsigned G = t.first[TAB], mine = t.first[(threadIdx.x & 63) + 1];
-    unsigned f = 0, l = 0;
-    long long n = 0;
-    double* p[NP] = {};
+    Finder<NP> at(t);
+    const unsigned G = t.first[Table<NP>::N];
     for (unsigned c = blockIdx.x; c < G; c += gridDim.x) {
         const unsigned q = REVERSE ? G - 1 - c : c;
-        if (q < f || q >= l) {
-            const int k = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine <= q)));
-            f = t.first[k];
-            l = t.first[k + 1];
-            n = t.n[k];
-#pragma unroll
-            for (int j = 0; j < NP; ++j) p[j] = t.p[j][k];
-        }
-        body(p, (long long)(q - f) * CHUNK, n);
+        at.find(q, CHUNK);
+        body(at.p, (long long)(q - at.f) * CHUNK, at.n);
     }
 }
 
@@ -149,7 +170,7 @@ template <int WAVES> __device__ __forceinline__ Part reduce_block(Part p) {
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = p;
     __syncthreads();
     Part r = sh[0];
-#pragma unroll
+#pragma unroll 3                   // (not all 16 parts in registers at once, next to the list that small_kernel keeps there)
     for (int w = 1; w < WAVES; ++w) join(r, sh[w]);
     return r;
 }
@@ -180,7 +201,7 @@ __device__ __forceinline__ void put_norms(const Norms& r, double* ws) { ws[0] = 
 template <bool CPLX, bool NT>
 __global__ __launch_bounds__(THREADS) void norm_partials_kernel(const Table<1> t, Part* out) {
     Acc acc;
-    chunks<1, false>(t, [&](double* const (&p)[1], long long a, long long n) {
+    chunks<1, false>(t, [&](double* const* p, long long a, long long n) {
         d2 v[UNROLL];
         load_chunk<NT>(v, p[0], a, n);
 #pragma unroll
@@ -216,7 +237,7 @@ __device__ __forceinline__ double factor(const Source& s) {
 template <bool NT>
 __global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const Source s) {
     const double c = factor(s);
-    chunks<2, true>(t, [&](double* const (&p)[2], long long a, long long n) {
+    chunks<2, true>(t, [&](double* const* p, long long a, long long n) {
         if (c == 1.0 && p[0] == p[1]) return;
         d2 v[UNROLL];
         load_chunk<false>(v, p[0], a, n);
@@ -239,7 +260,7 @@ template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d,
 template <bool MOMENTUM, bool NT>
 __global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 : 2> t, const Step s, const Source src) {
     const double c = factor(src);
-    chunks<MOMENTUM ? 3 : 2, true>(t, [&](double* const (&p)[MOMENTUM ? 3 : 2], long long a, long long n) {
+    chunks<MOMENTUM ? 3 : 2, true>(t, [&](double* const* p, long long a, long long n) {
         d2 x[UNROLL], d[UNROLL], m[UNROLL];
         load_chunk<false>(d, p[1], a, n);
         if (MOMENTUM && !s.first) load_chunk<false>(m, p[MOMENTUM ? 2 : 0], a, n);
@@ -251,10 +272,13 @@ __global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 :
     });
 }
 
-// Short lists: one workgroup, one launch, the list in registers between the norm and the second use.  Its 16 waves take pieces of 128 doubles.
+// Short lists: one workgroup, one launch, the list in registers between the norm and its second use.  Its 16 waves take pieces of 128 doubles,
+// ROUNDS of them each.
 constexpr int PIECE = 128, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
 enum { OP_NORMS, OP_CLIP, OP_SGD, OP_SGD_MOMENTUM };
-template <int OP> struct Shape { static constexpr int NP = OP == OP_NORMS ? 1 : OP == OP_SGD_MOMENTUM ? 3 : 2, READ = OP >= OP_SGD ? 1 : 0, ROUNDS = OP >= OP_SGD ? 4 : 8; };
+template <int OP> struct Shape {
+    static constexpr int NP = OP == OP_NORMS ? 1 : OP == OP_SGD_MOMENTUM ? 3 : 2, READ = OP >= OP_SGD ? 1 : 0, ROUNDS = OP == OP_NORMS ? 6 : 3;
+};
 
 __device__ __forceinline__ d2 load_piece(const double* x, int i, int n) {
     d2 v = {0.0, 0.0};
@@ -270,21 +294,20 @@ __device__ __forceinline__ void store_piece(d2 v, double* x, int i, int n) {
 template <int OP, bool CPLX>
 __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(const Table<Shape<OP>::NP> t, const Bound bd, const Step s, double* ws) {
     using S = Shape<OP>;
-    const unsigned G = t.first[TAB], lane = threadIdx.x & 63, mine = t.first[lane + 1];
+    Finder<S::NP> at(t);
+    const unsigned G = t.first[Table<S::NP>::N];
+    const int lane = threadIdx.x & 63;
     const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int k[S::ROUNDS], i[S::ROUNDS], n[S::ROUNDS];
     d2 v[S::ROUNDS], x[S::ROUNDS], m[S::ROUNDS];
 #pragma unroll
     for (int r = 0; r < S::ROUNDS; ++r) {
         const unsigned q = wave + r * SMALL_WAVES;
-        v[r] = d2{0.0, 0.0};
         if (q < G) {
-            k[r] = __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine <= q)));
-            i[r] = (int)(q - t.first[k[r]]) * PIECE + 2 * (int)lane;
-            n[r] = (int)t.n[k[r]];
-            v[r] = load_piece(t.p[S::READ][k[r]], i[r], n[r]);
-            if (OP >= OP_SGD) x[r] = load_piece(t.p[0][k[r]], i[r], n[r]);
-            if (OP == OP_SGD_MOMENTUM) m[r] = load_piece(t.p[S::NP - 1][k[r]], i[r], n[r]);
+            at.find(q, PIECE);
+            const int i = (int)(q - at.f) * PIECE + 2 * lane, n = (int)at.n;
+            v[r] = load_piece(at.p[S::READ], i, n);
+            if (OP >= OP_SGD) x[r] = load_piece(at.p[0], i, n);
+            if (OP == OP_SGD_MOMENTUM) m[r] = load_piece(at.p[S::NP - 1], i, n);
         }
     }
     Acc acc;
@@ -296,21 +319,23 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(const Table<Shape<
     if (OP == OP_NORMS) return;
 #pragma unroll
     for (int r = 0; r < S::ROUNDS; ++r) {
-        if (wave + r * SMALL_WAVES >= G) return;
+        const unsigned q = wave + r * SMALL_WAVES;
+        if (q >= G) return;
+        at.find(q, PIECE);
+        const int i = (int)(q - at.f) * PIECE + 2 * lane, n = (int)at.n;
         if (OP == OP_CLIP) {
-            double* y = t.p[S::NP - 1][k[r]];
-            if (nr.c != 1.0 || y != t.p[0][k[r]]) store_piece(v[r] * nr.c, y, i[r], n[r]);
+            if (nr.c != 1.0 || at.p[S::NP - 1] != at.p[0]) store_piece(v[r] * nr.c, at.p[S::NP - 1], i, n);
         } else {
             step_pair<OP == OP_SGD_MOMENTUM>(x[r], v[r], m[r], nr.c, s);
-            if (OP == OP_SGD_MOMENTUM) store_piece(v[r], t.p[S::NP - 1][k[r]], i[r], n[r]);
-            store_piece(x[r], t.p[0][k[r]], i[r], n[r]);
+            if (OP == OP_SGD_MOMENTUM) store_piece(v[r], at.p[S::NP - 1], i, n);
+            store_piece(x[r], at.p[0], i, n);
         }
     }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 
-// A list of nt tensors with NP pointers each, cut into launches of at most TAB non-empty tensors.
+// A list of nt tensors with NP pointers each
 template <int NP> struct Lists {
     int nt; const double* const* p[NP]; const long long* n; long long unit;      // unit: doubles per element
 };
@@ -368,17 +393,35 @@ template <int NP> int check_lists(ctm_ctx* ctx, const char* name, const Lists<NP
 }
 
 // The next launch's table from tensor `i` on; returns the index behind its last tensor.
+constexpr uintptr_t SPAN = (uintptr_t)8 << 32;           // what 32-bit counts of doubles reach
 template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t, int chunk = CHUNK) {
-    int k = 0;
-    unsigned q = 0;
-    for (; i < L.nt && k < TAB; ++i) {
+    constexpr int N = Table<NP>::N;
+    int take[N], k = 0;
+    uintptr_t lo[NP], hi[NP];
+    for (; i < L.nt && k < N; ++i) {
         if (!L.n[i]) continue;
-        for (int j = 0; j < NP; ++j) t.p[j][k] = const_cast<double*>(L.p[j][i]);
-        t.n[k] = L.n[i] * L.unit;
-        t.first[k++] = q;
-        q += (unsigned)((t.n[k - 1] + chunk - 1) / chunk);
+        bool fits = true;
+        uintptr_t a[NP], b[NP];
+        for (int j = 0; j < NP; ++j) {
+            const uintptr_t x = (uintptr_t)L.p[j][i];
+            a[j] = k && lo[j] < x ? lo[j] : x;
+            b[j] = k && hi[j] > x ? hi[j] : x;
+            fits &= b[j] - a[j] < SPAN;
+        }
+        if (!fits) break;                                // (never for the first tensor)
+        for (int j = 0; j < NP; ++j) { lo[j] = a[j]; hi[j] = b[j]; }
+        take[k++] = i;
     }
-    for (int j = k; j <= TAB; ++j) t.first[j] = q;
+    unsigned q = 0;
+    for (int j = 0; j < NP; ++j) t.base[j] = (double*)(k ? lo[j] : 0);
+    for (int e = 0; e < k; ++e) {
+        const long long n = L.n[take[e]] * L.unit, c = (n + chunk - 1) / chunk;
+        for (int j = 0; j < NP; ++j) t.offset[j][e] = (unsigned)(((uintptr_t)L.p[j][take[e]] - lo[j]) / 8);
+        t.first[e] = q;
+        t.tail[e] = (unsigned short)(n - (c - 1) * chunk - 1);
+        q += (unsigned)c;
+    }
+    for (int e = k; e <= N; ++e) t.first[e] = q;
     return i;
 }
 
@@ -408,7 +451,17 @@ Size size_of(const long long* n, int nt, long long unit) {
     }
     return s;
 }
-bool is_small(const Size& z, int rounds) { return z.tensors <= TAB && z.pieces <= rounds * SMALL_WAVES; }
+template <int OP> bool small(ctm_ctx* ctx, hipStream_t s, const Lists<Shape<OP>::NP>& L, const Size& z, Bound bd, const Step& st, double* ws, int* status) {
+    Table<Shape<OP>::NP> t;
+    if (z.tensors > t.N || z.pieces > Shape<OP>::ROUNDS * SMALL_WAVES) return false;
+    if (fill(L, 0, t, PIECE) < L.nt) return false;       // (tensors too far from each other)
+    *status = [&]() -> int {
+        if (ctx->cplx) GRADS_LAUNCH(ctx, s, (small_kernel<OP, true>), 1, SMALL_THREADS, t, bd, st, ws);
+        else GRADS_LAUNCH(ctx, s, (small_kernel<OP, false>), 1, SMALL_THREADS, t, bd, st, ws);
+        return CTM_OK;
+    }();
+    return true;
+}
 
 // Lists that do not fit the 256 MB last-level cache are read once without a claim on it (545 MB: 82 us against 87); stores of lists longer than
 // the 32 MB of L2 cache bypass it (545 MB scaled in 185 us against 188 ... 229, 1.1 GB after its norm pass in 556 against 591).
@@ -420,7 +473,7 @@ template <bool NT> int partials(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, 
     for (int i = 0; i < L.nt;) {
         Table<1> t;
         i = fill(L, i, t);
-        const unsigned long long g = t.first[TAB];
+        const unsigned long long g = t.first[t.N];
         if (!g) break;
         unsigned long long grid = z.chunks <= PARTIALS ? g : PARTIALS * g / z.chunks;
         if (grid < 1) grid = 1;
@@ -431,12 +484,8 @@ template <bool NT> int partials(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, 
     return CTM_OK;
 }
 
-template <int OP> int small(ctm_ctx* ctx, hipStream_t s, const Lists<Shape<OP>::NP>& L, Bound bd, const Step& st, double* ws) {
-    Table<Shape<OP>::NP> t;
-    fill(L, 0, t, PIECE);
-    if (ctx->cplx) GRADS_LAUNCH(ctx, s, (small_kernel<OP, true>), 1, SMALL_THREADS, t, bd, st, ws);
-    else GRADS_LAUNCH(ctx, s, (small_kernel<OP, false>), 1, SMALL_THREADS, t, bd, st, ws);
-    return CTM_OK;
+int norm_pass(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, double* ws, int* np) {
+    return z.bytes > LLC_BYTES ? partials<true>(ctx, s, L, z, ws, np) : partials<false>(ctx, s, L, z, ws, np);
 }
 
 // Second pass over a list: launch(table, grid, source) for every table of it.
@@ -445,7 +494,7 @@ template <int NP, class F> int second_pass(const Lists<NP>& L, Source src, F&& l
     for (int i = 0; i < L.nt;) {
         Table<NP> t;
         i = fill(L, i, t);
-        const unsigned g = t.first[TAB];
+        const unsigned g = t.first[t.N];
         if (!g) break;
         CTM_TRY(launch(t, g < MAX_GRID ? g : MAX_GRID, src));
         src.ws = nullptr;                    // the norms are written once
@@ -475,10 +524,9 @@ int ctm_grad_norms(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* 
     const Lists<1> L{nt, {x}, n, ctx->cplx ? 2 : 1};
     const Size z = size_of(n, nt, L.unit);
     const Bound none{-1.0, 0};
-    if (is_small(z, Shape<OP_NORMS>::ROUNDS)) return small<OP_NORMS>(ctx, s, L, none, Step{}, ws);
-    int np;
-    if (z.bytes > LLC_BYTES) CTM_TRY(partials<true>(ctx, s, L, z, ws, &np));
-    else CTM_TRY(partials<false>(ctx, s, L, z, ws, &np));
+    int status, np;
+    if (small<OP_NORMS>(ctx, s, L, z, none, Step{}, ws, &status)) return status;
+    CTM_TRY(norm_pass(ctx, s, L, z, ws, &np));
     GRADS_LAUNCH(ctx, s, norm_finish_kernel, 1, 1024, (const Part*)(ws + WS_HEAD), np, none, ws);
     return CTM_OK;
     });
@@ -497,9 +545,9 @@ int ctm_grad_clip(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x
     hipStream_t s = (hipStream_t)hip_stream;
     const Bound bd{max_norm, norm_type == CTM_NORM_INF};
     const Size z = size_of(n, nt, L.unit);
-    if (is_small(z, Shape<OP_CLIP>::ROUNDS)) return small<OP_CLIP>(ctx, s, L, bd, Step{}, ws);
-    int np;
-    CTM_TRY(partials<false>(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, ws, &np));
+    int status, np;
+    if (small<OP_CLIP>(ctx, s, L, z, bd, Step{}, ws, &status)) return status;
+    CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, ws, &np));
     return second_pass(L, Source{(const Part*)(ws + WS_HEAD), np, bd, ws}, [&](const Table<2>& t, unsigned grid, const Source& f) -> int {
         if (z.bytes > L2_BYTES) GRADS_LAUNCH(ctx, s, clip_kernel<true>, grid, THREADS, t, f);
         else GRADS_LAUNCH(ctx, s, clip_kernel<false>, grid, THREADS, t, f);
@@ -528,8 +576,9 @@ int ctm_sgd_step(ctm_ctx* ctx, void* hip_stream, int nt, double* const* p, const
     const Size z = size_of(n, nt, L2.unit);
     Source src{nullptr, 0, Bound{bounded ? max_norm : -1.0, norm_type == CTM_NORM_INF}, ws};
     if (bounded) {
-        if (is_small(z, Shape<OP_SGD>::ROUNDS)) return m ? small<OP_SGD_MOMENTUM>(ctx, s, L3, src.bd, st, ws) : small<OP_SGD>(ctx, s, L2, src.bd, st, ws);
-        CTM_TRY(partials<false>(ctx, s, Lists<1>{nt, {g}, n, L2.unit}, z, ws, &src.np));
+        int status;
+        if (m ? small<OP_SGD_MOMENTUM>(ctx, s, L3, z, src.bd, st, ws, &status) : small<OP_SGD>(ctx, s, L2, z, src.bd, st, ws, &status)) return status;
+        CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {g}, n, L2.unit}, z, ws, &src.np));
         src.part = (const Part*)(ws + WS_HEAD);
     }
     return m ? sgd<true>(ctx, s, L3, z, st, src) : sgd<false>(ctx, s, L2, z, st, src);
