@@ -308,7 +308,7 @@ int ctm_init_piece(ctm_ctx* ctx, int kind, const double* a, const int* adims, do
  *     ws[2] = c = 1 if the chosen norm <= max_norm, else max_norm / norm (NaN norm: NaN; infinite norm: 0)
  * (0, 0, 1 for an empty list; NaN in the list: both NaN).  Sums have a fixed order: equal inputs give equal bits.
  * Memory that is written must not overlap any other range of the call (clip: y[i] == x[i] is allowed): CTM_ERR_BADARG. */
-#define CTM_GRAD_WS_DOUBLES(nt) (4 * (1025 + (nt)))
+#define CTM_GRAD_WS_DOUBLES(nt) (4 * (1089 + 16 * (nt)))
 enum { CTM_NORM_INF = 0, CTM_NORM_2 = 2 };
 int ctm_grad_norms(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x, const long long* n, double* ws, long long ws_doubles);
 /* y[i] = c x[i]; in place (y[i] == x[i]) a list inside the bound keeps its bits */

@@ -1003,7 +1003,7 @@ class Engine:
                 call()
 
     def _grad_ws(self, nt):
-        return torch.empty(4 * (1025 + nt), dtype=torch.float64, device=self.device)          # CTM_GRAD_WS_DOUBLES(nt)
+        return torch.empty(4 * (1089 + 16 * nt), dtype=torch.float64, device=self.device)          # CTM_GRAD_WS_DOUBLES(nt)
 
     @staticmethod
     def _norm_code(what, norm_type):

@@ -11,7 +11,7 @@ import os, subprocess, sys, shutil
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 SOURCES = ["ctm_runtime.hip", "gemm_f64.hip", "tensor_ops.hip", "jacobi_core.hip", "svd_leading.hip", "eigh.hip", "contract.hip", "layer2.hip", "ctm_ops.hip", "backward.hip", "ctm_move.hip", "grads.hip"]
-HEADERS = ["ctm_common.h", "contract.h", "jacobi_internal.h", os.path.join("..", "..", "include", "ctm_hip.h")]
+HEADERS = ["ctm_common.h", "contract.h", "jacobi_internal.h", "grads_lists.h", os.path.join("..", "..", "include", "ctm_hip.h")]
 # Python module that reads lists of tensors (host code only, against torch's own headers)
 EXT_SOURCE = os.path.join(HERE, "lists.cpp")
 EXT = os.path.join(PKG, "_ctm_lists.so")

@@ -7,27 +7,9 @@
 // All of it is bound by memory traffic on long lists (3 ... 9 flop per 8 ... 40 bytes) and by launches on short ones.  Nothing is kept between
 // calls, nothing is read back by the host, no atomics and no memset: every sum has a fixed order, and a captured call replays as it ran.
 #include "ctm_common.h"
-#include <algorithm>
+#include "grads_lists.h"
 
 namespace {
-
-constexpr int THREADS = 256;
-constexpr int UNROLL = 4;              // 16-byte loads in flight per thread
-constexpr int CHUNK = 2 * THREADS * UNROLL;      // doubles: what a workgroup takes at a time; a chunk lies in one tensor
-constexpr int WS_HEAD = 4;             // ws: N2, Ninf, c, unused, then the partial results (4 doubles each)
-constexpr int PARTIALS = 1024;         // workgroups of the norm pass over all launches, up to one more per launch
-
-// The tensors of one launch.  Their table travels by value in the kernel arguments (no host-to-device copy, so a call may be captured), which hold
-// 4 kB: addresses are 32-bit counts of doubles above the lowest one (tensors of a launch lie within 32 GB), lengths what the last chunk holds.
-// More tensors per launch, fewer launches -- each costs >= 4 us, more than the work on a hundred short tensors.
-template <int NP> struct Table {
-    static constexpr int N = NP == 1 ? 384 : NP == 2 ? 256 : 192;
-    double* base[NP];
-    unsigned offset[NP][N];
-    unsigned first[N + 1];             // chunks before tensor t; entries behind the last tensor hold the total
-    unsigned short tail[N];            // doubles of the last chunk, less one (a complex element counts two)
-};
-static_assert(sizeof(Table<1>) <= 3968 && sizeof(Table<2>) <= 3968 && sizeof(Table<3>) <= 3968, "the kernel arguments hold 4 kB");
 
 typedef double d2 __attribute__((ext_vector_type(2)));
 typedef d2 d2u __attribute__((aligned(8)));          // 16-byte access at 8-byte alignment: views into a flat buffer start anywhere
@@ -64,18 +46,17 @@ template <int NP> struct Finder {
         l = t.first[k + 1];
         n = (long long)(l - f - 1) * chunk + t.tail[k] + 1;
 #pragma unroll
-        for (int j = 0; j < NP; ++j) p[j] = t.base[j] + t.offset[j][k];
+        for (int j = 0; j < NP; ++j) p[j] = t.base[j][(t.which[k] >> (2 * j)) & 3] + t.offset[j][k];
     }
 };
 
 // Runs body(pointers, first double, length of the tensor) over this workgroup's chunks: every gridDim.x-th one, so that all workgroups sweep the
 // list together (measured on 545 MB: 87 us for the norm pass against 95 with one contiguous share per workgroup, 185 against 223 for the
-// scaling).  REVERSE: from the list's end to its beginning -- a second pass meets first what the pass before it left in the 256 MB last-level cache.
-template <int NP, bool REVERSE, class F> __device__ __forceinline__ void chunks(const Table<NP>& t, F&& body) {
+// scaling).
+template <int NP, class F> __device__ __forceinline__ void chunks(const Table<NP>& t, F&& body) {
     Finder<NP> at(t);
     const unsigned G = t.first[Table<NP>::N];
-    for (unsigned c = blockIdx.x; c < G; c += gridDim.x) {
-        const unsigned q = REVERSE ? G - 1 - c : c;
+    for (unsigned q = blockIdx.x; q < G; q += gridDim.x) {
         at.find(q, CHUNK);
         body(at.p, (long long)(q - at.f) * CHUNK, at.n);
     }
@@ -201,7 +182,7 @@ __device__ __forceinline__ void put_norms(const Norms& r, double* ws) { ws[0] = 
 template <bool CPLX, bool NT>
 __global__ __launch_bounds__(THREADS) void norm_partials_kernel(const Table<1> t, Part* out) {
     Acc acc;
-    chunks<1, false>(t, [&](double* const* p, long long a, long long n) {
+    chunks<1>(t, [&](double* const* p, long long a, long long n) {
         d2 v[UNROLL];
         load_chunk<NT>(v, p[0], a, n);
 #pragma unroll
@@ -223,13 +204,13 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const Part* part, int
     if (threadIdx.x == 0) put_norms(r, ws);
 }
 
-// Where the second pass gets its factor from: every workgroup joins the partial results by itself (32 kB at most, from the L2 cache; all get the
-// same bits), which is cheaper than a kernel in between.
-struct Source { const Part* part; int np; Bound bd; double* ws; };      // ws: the norms are written there (by one workgroup); may be null
+// Where the second pass gets its factor from: every workgroup joins the partial results by itself (32 kB from the L2 cache; all get the same bits),
+// which is as fast as a kernel in between on long lists and saves its 4 us on short ones.
+struct Source { const Part* part; int np; Bound bd; double* ws; bool write; };      // write: one workgroup leaves the norms in ws
 __device__ __forceinline__ double factor(const Source& s) {
     if (s.bd.max_norm < 0.0) return 1.0;
     const Norms r = join_partials<THREADS>(s.part, s.np, s.bd);
-    if (s.ws && blockIdx.x == 0 && threadIdx.x == 0) put_norms(r, s.ws);
+    if (s.write && blockIdx.x == 0 && threadIdx.x == 0) put_norms(r, s.ws);
     return r.c;
 }
 
@@ -237,7 +218,7 @@ __device__ __forceinline__ double factor(const Source& s) {
 template <bool NT>
 __global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const Source s) {
     const double c = factor(s);
-    chunks<2, true>(t, [&](double* const* p, long long a, long long n) {
+    chunks<2>(t, [&](double* const* p, long long a, long long n) {
         if (c == 1.0 && p[0] == p[1]) return;
         d2 v[UNROLL];
         load_chunk<false>(v, p[0], a, n);
@@ -260,7 +241,7 @@ template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d,
 template <bool MOMENTUM, bool NT>
 __global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 : 2> t, const Step s, const Source src) {
     const double c = factor(src);
-    chunks<MOMENTUM ? 3 : 2, true>(t, [&](double* const* p, long long a, long long n) {
+    chunks<MOMENTUM ? 3 : 2>(t, [&](double* const* p, long long a, long long n) {
         d2 x[UNROLL], d[UNROLL], m[UNROLL];
         load_chunk<false>(d, p[1], a, n);
         if (MOMENTUM && !s.first) load_chunk<false>(m, p[MOMENTUM ? 2 : 0], a, n);
@@ -274,7 +255,7 @@ __global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 :
 
 // Short lists: one workgroup, one launch, the list in registers between the norm and its second use.  Its 16 waves take pieces of 128 doubles,
 // ROUNDS of them each.
-constexpr int PIECE = 128, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
+constexpr int SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
 enum { OP_NORMS, OP_CLIP, OP_SGD, OP_SGD_MOMENTUM };
 template <int OP> struct Shape {
     static constexpr int NP = OP == OP_NORMS ? 1 : OP == OP_SGD_MOMENTUM ? 3 : 2, READ = OP >= OP_SGD ? 1 : 0, ROUNDS = OP == OP_NORMS ? 6 : 3;
@@ -335,11 +316,6 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(const Table<Shape<
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 
-// A list of nt tensors with NP pointers each
-template <int NP> struct Lists {
-    int nt; const double* const* p[NP]; const long long* n; long long unit;      // unit: doubles per element
-};
-
 int list_error(ctm_ctx* ctx, const char* name, const std::string& what) {
     ctx->set_error(std::string(name) + ": " + what);
     return CTM_ERR_BADARG;
@@ -350,79 +326,6 @@ int check_device(ctm_ctx* ctx, const char* name) {
     CTM_HIP_CHECK(ctx, hipGetDevice(&dev));
     if (dev != ctx->device) return list_error(ctx, name, "the context belongs to device " + std::to_string(ctx->device) + ", device " + std::to_string(dev) + " is current");
     return CTM_OK;
-}
-
-// Lengths, pointers and the memory that is written: no written range may overlap any other range of the call (in a clip the range that is read
-// and written under the same index may be one and the same).
-template <int NP> int check_lists(ctm_ctx* ctx, const char* name, const Lists<NP>& L, const bool (&written)[NP], int same_as_first) {
-    if (L.nt < 0) return list_error(ctx, name, "negative number of tensors");
-    if (L.nt && !L.n) return list_error(ctx, name, "lengths missing");
-    for (int j = 0; j < NP; ++j) if (L.nt && !L.p[j]) return list_error(ctx, name, "pointers missing");
-    long long total = 0;
-    bool any_written = false;
-    for (int i = 0; i < L.nt; ++i) {
-        if (L.n[i] < 0 || L.n[i] > (1LL << 40)) return list_error(ctx, name, "length of tensor " + std::to_string(i) + " out of range");
-        total += L.n[i];
-        if (total > (1LL << 40)) return list_error(ctx, name, "list too long");
-        if (!L.n[i]) continue;
-        for (int j = 0; j < NP; ++j) {
-            if (!L.p[j][i]) return list_error(ctx, name, "null pointer for tensor " + std::to_string(i));
-            if ((uintptr_t)L.p[j][i] % 8) return list_error(ctx, name, "tensor " + std::to_string(i) + " is not aligned to 8 bytes");
-        }
-    }
-    for (int j = 0; j < NP; ++j) any_written |= written[j];
-    if (!any_written) return CTM_OK;
-    struct Range { uintptr_t a, b; bool w; };
-    std::vector<Range> r;
-    r.reserve((size_t)NP * L.nt);
-    for (int i = 0; i < L.nt; ++i)
-        for (int j = 0; j < NP; ++j) {
-            if (!L.n[i] || (j > 0 && j == same_as_first && L.p[j][i] == L.p[0][i])) continue;
-            const uintptr_t a = (uintptr_t)L.p[j][i];
-            const bool w = written[j] || (j == 0 && same_as_first > 0 && L.p[same_as_first][i] == L.p[0][i]);
-            r.push_back({a, a + (uintptr_t)(8 * L.unit * L.n[i]), w});
-        }
-    std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.a < y.a; });
-    uintptr_t end_any = 0, end_written = 0;
-    for (const Range& x : r) {
-        if (x.a < end_written || (x.w && x.a < end_any)) return list_error(ctx, name, "a tensor that is written overlaps another tensor of the call");
-        if (x.b > end_any) end_any = x.b;
-        if (x.w && x.b > end_written) end_written = x.b;
-    }
-    return CTM_OK;
-}
-
-// The next launch's table from tensor `i` on; returns the index behind its last tensor.
-constexpr uintptr_t SPAN = (uintptr_t)8 << 32;           // what 32-bit counts of doubles reach
-template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t, int chunk = CHUNK) {
-    constexpr int N = Table<NP>::N;
-    int take[N], k = 0;
-    uintptr_t lo[NP], hi[NP];
-    for (; i < L.nt && k < N; ++i) {
-        if (!L.n[i]) continue;
-        bool fits = true;
-        uintptr_t a[NP], b[NP];
-        for (int j = 0; j < NP; ++j) {
-            const uintptr_t x = (uintptr_t)L.p[j][i];
-            a[j] = k && lo[j] < x ? lo[j] : x;
-            b[j] = k && hi[j] > x ? hi[j] : x;
-            fits &= b[j] - a[j] < SPAN;
-        }
-        if (!fits) break;                                // (never for the first tensor)
-        for (int j = 0; j < NP; ++j) { lo[j] = a[j]; hi[j] = b[j]; }
-        take[k++] = i;
-    }
-    unsigned q = 0;
-    for (int j = 0; j < NP; ++j) t.base[j] = (double*)(k ? lo[j] : 0);
-    for (int e = 0; e < k; ++e) {
-        const long long n = L.n[take[e]] * L.unit, c = (n + chunk - 1) / chunk;
-        for (int j = 0; j < NP; ++j) t.offset[j][e] = (unsigned)(((uintptr_t)L.p[j][take[e]] - lo[j]) / 8);
-        t.first[e] = q;
-        t.tail[e] = (unsigned short)(n - (c - 1) * chunk - 1);
-        q += (unsigned)c;
-    }
-    for (int e = k; e <= N; ++e) t.first[e] = q;
-    return i;
 }
 
 // launch on the caller's stream, CTM_LAUNCH's checks
@@ -438,19 +341,6 @@ template <int NP> int fill(const Lists<NP>& L, int i, Table<NP>& t, int chunk = 
         }                                                                                                         \
     } while (0)
 
-// What the choice of a kernel goes by: chunks and bytes of the list, whether one workgroup takes all of it
-struct Size { unsigned chunks; int tensors; long long pieces, bytes; };
-Size size_of(const long long* n, int nt, long long unit) {
-    Size s{0, 0, 0, 0};
-    for (int i = 0; i < nt; ++i) {
-        const long long d = n[i] * unit;
-        s.chunks += (unsigned)((d + CHUNK - 1) / CHUNK);
-        s.pieces += (d + PIECE - 1) / PIECE;
-        s.tensors += d > 0;
-        s.bytes += 8 * d;
-    }
-    return s;
-}
 template <int OP> bool small(ctm_ctx* ctx, hipStream_t s, const Lists<Shape<OP>::NP>& L, const Size& z, Bound bd, const Step& st, double* ws, int* status) {
     Table<Shape<OP>::NP> t;
     if (z.tensors > t.N || z.pieces > Shape<OP>::ROUNDS * SMALL_WAVES) return false;
@@ -463,41 +353,46 @@ template <int OP> bool small(ctm_ctx* ctx, hipStream_t s, const Lists<Shape<OP>:
     return true;
 }
 
-// Lists that do not fit the 256 MB last-level cache are read once without a claim on it (545 MB: 82 us against 87); stores of lists longer than
-// the 32 MB of L2 cache bypass it (545 MB scaled in 185 us against 188 ... 229, 1.1 GB after its norm pass in 556 against 591).
+// Lists that do not fit the 256 MB last-level cache are read by the norm pass without a claim on it (545 MB: 82 us against 87); stores of lists longer
+// than the 32 MB of L2 cache bypass it (545 MB scaled in 185 us against 188 ... 229).
 constexpr long long LLC_BYTES = 256LL << 20, L2_BYTES = 32LL << 20;
 
-template <bool NT> int partials(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, double* ws, int* np) {
-    *np = 0;
+// The norm pass; the partial results are at ws + WS_HEAD
+int norm_pass(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, double* ws, int* count) {
     Part* part = (Part*)(ws + WS_HEAD);
+    int np = 0;
     for (int i = 0; i < L.nt;) {
         Table<1> t;
         i = fill(L, i, t);
-        const unsigned long long g = t.first[t.N];
+        const unsigned g = t.first[t.N];
         if (!g) break;
-        unsigned long long grid = z.chunks <= PARTIALS ? g : PARTIALS * g / z.chunks;
-        if (grid < 1) grid = 1;
-        if (ctx->cplx) GRADS_LAUNCH(ctx, s, (norm_partials_kernel<true, NT>), (unsigned)grid, THREADS, t, part + *np);
-        else GRADS_LAUNCH(ctx, s, (norm_partials_kernel<false, NT>), (unsigned)grid, THREADS, t, part + *np);
-        *np += (int)grid;
+        unsigned grid = PARTIALS_LEAST + (unsigned)((unsigned long long)PARTIALS * g / z.chunks);
+        grid = grid > PARTIALS ? PARTIALS : grid;
+        grid = grid > g ? g : grid;
+        if (z.bytes > LLC_BYTES) {
+            if (ctx->cplx) GRADS_LAUNCH(ctx, s, (norm_partials_kernel<true, true>), grid, THREADS, t, part + np);
+            else GRADS_LAUNCH(ctx, s, (norm_partials_kernel<false, true>), grid, THREADS, t, part + np);
+        } else {
+            if (ctx->cplx) GRADS_LAUNCH(ctx, s, (norm_partials_kernel<true, false>), grid, THREADS, t, part + np);
+            else GRADS_LAUNCH(ctx, s, (norm_partials_kernel<false, false>), grid, THREADS, t, part + np);
+        }
+        np += (int)grid;
     }
+    *count = np;
     return CTM_OK;
 }
 
-int norm_pass(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, double* ws, int* np) {
-    return z.bytes > LLC_BYTES ? partials<true>(ctx, s, L, z, ws, np) : partials<false>(ctx, s, L, z, ws, np);
-}
-
-// Second pass over a list: launch(table, grid, source) for every table of it.
-constexpr unsigned MAX_GRID = 8192;
+// Second pass over a list: launch(table, workgroups, source) for every table of it.  One workgroup per chunk: the table's lookup and the joining of
+// the partial results cost less than the tail of a grid that walks (1.1 GB clipped: 535 us against 553 with 8192 workgroups, 569 with 2048).
+constexpr unsigned MOST = 1u << 23;          // (a grid holds at most 2^32 threads)
 template <int NP, class F> int second_pass(const Lists<NP>& L, Source src, F&& launch) {
     for (int i = 0; i < L.nt;) {
         Table<NP> t;
         i = fill(L, i, t);
         const unsigned g = t.first[t.N];
         if (!g) break;
-        CTM_TRY(launch(t, g < MAX_GRID ? g : MAX_GRID, src));
-        src.ws = nullptr;                    // the norms are written once
+        CTM_TRY(launch(t, g < MOST ? g : MOST, src));
+        src.write = false;                   // the norms are written once
     }
     return CTM_OK;
 }
@@ -518,14 +413,15 @@ int ctm_grad_norms(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* 
     return ctm_entry(ctx, "ctm_grad_norms", [&]() -> int {
     CTM_TRY(check_device(ctx, "grad_norms"));
     const bool written[1] = {false};
-    CTM_TRY(check_lists<1>(ctx, "grad_norms", Lists<1>{nt, {x}, n, ctx->cplx ? 2 : 1}, written, 0));
+    if (const std::string e = check_lists(Lists<1>{nt, {x}, n, ctx->cplx ? 2 : 1}, written, 0); !e.empty()) return list_error(ctx, "grad_norms", e);
     if (!ws || ws_doubles < CTM_GRAD_WS_DOUBLES((long long)nt)) return list_error(ctx, "grad_norms", "workspace too small (CTM_GRAD_WS_DOUBLES)");
     hipStream_t s = (hipStream_t)hip_stream;
     const Lists<1> L{nt, {x}, n, ctx->cplx ? 2 : 1};
     const Size z = size_of(n, nt, L.unit);
     const Bound none{-1.0, 0};
-    int status, np;
+    int status;
     if (small<OP_NORMS>(ctx, s, L, z, none, Step{}, ws, &status)) return status;
+    int np;
     CTM_TRY(norm_pass(ctx, s, L, z, ws, &np));
     GRADS_LAUNCH(ctx, s, norm_finish_kernel, 1, 1024, (const Part*)(ws + WS_HEAD), np, none, ws);
     return CTM_OK;
@@ -538,17 +434,18 @@ int ctm_grad_clip(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x
     CTM_TRY(check_device(ctx, "grad_clip"));
     const bool written[2] = {false, true};
     Lists<2> L{nt, {x, (const double* const*)y}, n, ctx->cplx ? 2 : 1};
-    CTM_TRY(check_lists<2>(ctx, "grad_clip", L, written, 1));
+    if (const std::string e = check_lists(L, written, 1); !e.empty()) return list_error(ctx, "grad_clip", e);
     if (!(max_norm >= 0.0)) return list_error(ctx, "grad_clip", "max_norm must be >= 0");
     if (norm_type != CTM_NORM_2 && norm_type != CTM_NORM_INF) return list_error(ctx, "grad_clip", "norm_type must be CTM_NORM_2 or CTM_NORM_INF");
     if (!ws || ws_doubles < CTM_GRAD_WS_DOUBLES((long long)nt)) return list_error(ctx, "grad_clip", "workspace too small (CTM_GRAD_WS_DOUBLES)");
     hipStream_t s = (hipStream_t)hip_stream;
     const Bound bd{max_norm, norm_type == CTM_NORM_INF};
     const Size z = size_of(n, nt, L.unit);
-    int status, np;
+    int status;
+    Source src{(const Part*)(ws + WS_HEAD), 0, bd, ws, true};
     if (small<OP_CLIP>(ctx, s, L, z, bd, Step{}, ws, &status)) return status;
-    CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, ws, &np));
-    return second_pass(L, Source{(const Part*)(ws + WS_HEAD), np, bd, ws}, [&](const Table<2>& t, unsigned grid, const Source& f) -> int {
+    CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, ws, &src.np));
+    return second_pass(L, src, [&](const Table<2>& t, unsigned grid, const Source& f) -> int {
         if (z.bytes > L2_BYTES) GRADS_LAUNCH(ctx, s, clip_kernel<true>, grid, THREADS, t, f);
         else GRADS_LAUNCH(ctx, s, clip_kernel<false>, grid, THREADS, t, f);
         return CTM_OK;
@@ -562,8 +459,8 @@ int ctm_sgd_step(ctm_ctx* ctx, void* hip_stream, int nt, double* const* p, const
     CTM_TRY(check_device(ctx, "sgd_step"));
     Lists<3> L3{nt, {(const double* const*)p, g, (const double* const*)m}, n, ctx->cplx ? 2 : 1};
     Lists<2> L2{nt, {(const double* const*)p, g}, n, ctx->cplx ? 2 : 1};
-    if (m) { const bool w[3] = {true, false, true}; CTM_TRY(check_lists<3>(ctx, "sgd_step", L3, w, 0)); }
-    else { const bool w[2] = {true, false}; CTM_TRY(check_lists<2>(ctx, "sgd_step", L2, w, 0)); }
+    const bool w3[3] = {true, false, true}, w2[2] = {true, false};
+    if (const std::string e = m ? check_lists(L3, w3, 0) : check_lists(L2, w2, 0); !e.empty()) return list_error(ctx, "sgd_step", e);
     if (nt > 0 && !m && momentum != 0.0) return list_error(ctx, "sgd_step", "momentum needs the momentum buffers");
     hipStream_t s = (hipStream_t)hip_stream;
     const bool bounded = max_norm >= 0.0;
@@ -574,12 +471,12 @@ int ctm_sgd_step(ctm_ctx* ctx, void* hip_stream, int nt, double* const* p, const
     }
     const Step st{lr, momentum, 1.0 - dampening, first};
     const Size z = size_of(n, nt, L2.unit);
-    Source src{nullptr, 0, Bound{bounded ? max_norm : -1.0, norm_type == CTM_NORM_INF}, ws};
+    const Bound bd{bounded ? max_norm : -1.0, norm_type == CTM_NORM_INF};
+    Source src{(const Part*)(ws + WS_HEAD), 0, bd, ws, true};          // (no bound: none of it is read)
     if (bounded) {
         int status;
-        if (m ? small<OP_SGD_MOMENTUM>(ctx, s, L3, z, src.bd, st, ws, &status) : small<OP_SGD>(ctx, s, L2, z, src.bd, st, ws, &status)) return status;
+        if (m ? small<OP_SGD_MOMENTUM>(ctx, s, L3, z, bd, st, ws, &status) : small<OP_SGD>(ctx, s, L2, z, bd, st, ws, &status)) return status;
         CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {g}, n, L2.unit}, z, ws, &src.np));
-        src.part = (const Part*)(ws + WS_HEAD);
     }
     return m ? sgd<true>(ctx, s, L3, z, st, src) : sgd<false>(ctx, s, L2, z, st, src);
     });

@@ -1,7 +1,7 @@
 // _ctm_lists: the short way from a Python list of tensors to the C entries over lists (ctm_grad_norms, ctm_grad_clip, ctm_sgd_step).  What those
 // entries cost on the lists of an optimisation is mostly the host's reading of pointers, dtypes and layouts: ten Python attribute accesses per
 // tensor are ~0.8 us, this module needs ~0.03 us.  It takes the plain case -- contiguous tensors of one dtype on one device -- and returns None for
-// everything else, refused arguments included; the caller (_native.py) then goes its general way, which handles strided views and words the errors.
+// everything else, refused arguments included (the interpreter's lock is held all along: nobody changes a list meanwhile); the caller (_native.py) then goes its general way, which handles strided views and words the errors.
 #include <torch/csrc/Device.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
@@ -70,15 +70,6 @@ PyObject* norms_of(at::Tensor&& ws) {
     return THPVariable_Wrap(std::move(ws));
 }
 
-// Status of a call, without the GIL
-template <class F> int status_of(F&& call) {
-    int st;
-    Py_BEGIN_ALLOW_THREADS
-    st = call();
-    Py_END_ALLOW_THREADS
-    return st;
-}
-
 // What a call that did not succeed gives: an argument that the entry refused goes the general way (nothing was launched), any other status is
 // returned as a number.
 PyObject* failed(int st) {
@@ -116,9 +107,7 @@ PyObject* grad_norms(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     List x;
     if (read(c, a[5], x, nullptr)) {
         at::Tensor ws = workspace(c, x.n);
-        const int st = status_of([&] {
-            return ((norms_fn)c.fn)(c.context(), c.stream, (int)x.n, x.ptr.data(), x.numel.data(), ws.mutable_data_ptr<double>(), ws.numel());
-        });
+        const int st = ((norms_fn)c.fn)(c.context(), c.stream, (int)x.n, x.ptr.data(), x.numel.data(), ws.mutable_data_ptr<double>(), ws.numel());
         return st == CTM_OK ? norms_of(std::move(ws)) : failed(st);
     }
     END_ENTRY
@@ -134,10 +123,8 @@ PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         const double bound = PyFloat_AsDouble(a[8]);
         if (PyErr_Occurred()) return nullptr;
         at::Tensor ws = workspace(c, x.n);
-        const int st = status_of([&] {
-            return ((clip_fn)c.fn)(c.context(), c.stream, (int)x.n, x.ptr.data(), const_cast<double* const*>(out.ptr.data()), x.numel.data(), code, bound,
-                                   ws.mutable_data_ptr<double>(), ws.numel());
-        });
+        const int st = ((clip_fn)c.fn)(c.context(), c.stream, (int)x.n, x.ptr.data(), const_cast<double* const*>(out.ptr.data()), x.numel.data(), code,
+                                       bound, ws.mutable_data_ptr<double>(), ws.numel());
         if (st != CTM_OK) return failed(st);
         changed(out);
         return norms_of(std::move(ws));
@@ -156,11 +143,9 @@ PyObject* sgd_step(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         if (PyErr_Occurred()) return nullptr;
         at::Tensor ws;
         if (bound >= 0.0) ws = workspace(c, p.n);
-        const int st = status_of([&] {
-            return ((sgd_fn)c.fn)(c.context(), c.stream, (int)p.n, const_cast<double* const*>(p.ptr.data()), g.ptr.data(),
-                                  buffers ? const_cast<double* const*>(m.ptr.data()) : nullptr, p.numel.data(), lr, mu, tau, first, code, bound,
-                                  ws.defined() ? ws.mutable_data_ptr<double>() : nullptr, ws.defined() ? ws.numel() : 0);
-        });
+        const int st = ((sgd_fn)c.fn)(c.context(), c.stream, (int)p.n, const_cast<double* const*>(p.ptr.data()), g.ptr.data(),
+                                      buffers ? const_cast<double* const*>(m.ptr.data()) : nullptr, p.numel.data(), lr, mu, tau, first, code, bound,
+                                      ws.defined() ? ws.mutable_data_ptr<double>() : nullptr, ws.defined() ? ws.numel() : 0);
         if (st != CTM_OK) return failed(st);
         changed(p);
         if (buffers) changed(m);

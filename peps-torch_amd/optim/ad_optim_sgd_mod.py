@@ -13,6 +13,8 @@ class SGD(torch.optim.Optimizer):
     without `max_norm`.  One parameter group, whose lr, momentum, dampening and max_norm may be changed between steps; a graph that captured
     a step keeps those of the capture, and is captured after the first step (which makes the momentum buffers)."""
 
+    norms = None
+
     def __init__(self, params, lr, momentum=0.0, dampening=0.0, max_norm=None, norm_type=2):
         for k, v in (("lr", lr), ("momentum", momentum), ("max_norm", 0.0 if max_norm is None else max_norm)):
             if not v >= 0.0:
@@ -22,7 +24,6 @@ class SGD(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, momentum=momentum, dampening=dampening, max_norm=max_norm, norm_type=norm_type))
         if len(self.param_groups) != 1:
             raise ValueError("SGD: one parameter group only (the norm is that of all parameters)")
-        self.norms = None
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -10,7 +10,7 @@ without limit next to degenerate singular values (linalg/svd_gesdd.py:209-328 re
 
 All tensors of a list are on one device and of one dtype; empty tensors, 0-dimensional tensors, strided views and empty lists are allowed.  A NaN
 anywhere makes both norms NaN and a clipped list all NaN; an infinite element makes c = 0 (0 x inf = NaN).  Calls run on the current stream, do not
-synchronise and may be captured into a graph (after one call outside of it, which makes the native context)."""
+synchronise and may be captured into a graph (after one call outside of it, which makes the native context); they are not differentiable."""
 from backend import get_engine
 
 

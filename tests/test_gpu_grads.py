@@ -76,8 +76,8 @@ LISTS = {
     "chunks": [4095, 4096, 8191, 8193],
     "empties_between": [0, 5, 0, 0, 513, 0], "pieces": [127, 128, 129, 255], "one_group": [16384], "one_group_half": [8192], "one_group_quarter": [4096],
     "group_of_many": [256] * 63 + [255], "group_and_one": [16383, 1], "over_group": [16385], "cell_D4": [512] * 4, "cell_D8": [8192] * 8,
-    "table_full": [3] * 64, "table_over": [5] * 65, "many": [(37 * i) % 411 for i in range(300)], "long": [1 << 20, 3, 777777],
-    "one_long": [5000001],
+    "table_full": [3] * 64, "table_over": [5] * 65, "many": [(37 * i) % 411 for i in range(300)], "long": [1 << 19, 3, 277777],
+    "one_long": [1500001],
 }
 
 
@@ -144,6 +144,60 @@ def test_step_of_lists(eng, name, dtype, mu, tau, first, max_ratio):
     if not mu:
         for t, a in zip(ms, m0):
             assert np.array_equal(t.cpu().numpy(), a)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lists_longer_than_the_caches(eng, dtype):
+    """Whole numbers and factors of 1/2, so that every product and sum is exact: the results equal torch's bit for bit.  0.37 GB, of odd lengths at
+    odd places."""
+    u = 2 if dtype == C128 else 1
+    lens = [35000003 // u, 5, 9000001 // u, 2048, 2300001 // u]
+    flat = torch.randint(-3, 4, (sum(lens) + 7, u), device="cuda", generator=torch.Generator("cuda").manual_seed(11)).to(F64)
+    flat = torch.view_as_complex(flat) if u == 2 else flat[:, 0]
+    cut = lambda t: list(t[1:1 + sum(lens)].split(lens))              # noqa: E731
+    squares = sum(int((torch.view_as_real(t) if u == 2 else t).to(torch.int64).pow(2).sum()) for t in cut(flat))
+    n2 = math.sqrt(squares)                                           # (sums of whole numbers below 2^53: exact in any order)
+    top = 3.0 * math.sqrt(u)
+    got = G.grad_norms(cut(flat)).tolist()
+    assert got[0] == n2 and abs(got[1] / top - 1) <= O.tol_top(u == 2)
+    out = torch.full_like(flat, 9.0)
+    assert G.clip_grads(cut(flat), n2 / 2, out=cut(out)).tolist() == got
+    assert torch.equal(torch.cat(cut(out)), torch.cat(cut(flat)) * 0.5)
+    assert bool((out[:1] == 9.0).all()) and bool((out[1 + sum(lens):] == 9.0).all())
+    p, m = flat.flip(0).contiguous(), (flat * 4).contiguous()
+    wm = 0.5 * m + 0.75 * (0.5 * flat)
+    wp = p - 0.25 * wm
+    for t, w in ((wp, p), (wm, m)):
+        t[:1], t[1 + sum(lens):] = w[:1], w[1 + sum(lens):]
+    assert G.sgd_step(cut(p), cut(flat), cut(m), lr=0.25, momentum=0.5, dampening=0.25, max_norm=n2 / 2).tolist() == got
+    assert torch.equal(p, wp) and torch.equal(m, wm)
+    q = p.clone()
+    G.sgd_step(cut(q), cut(flat), lr=0.25)
+    wp = p - 0.25 * flat
+    wp[:1], wp[1 + sum(lens):] = p[:1], p[1 + sum(lens):]
+    assert torch.equal(q, wp)
+    G.clip_grads(cut(flat), n2 / 2)                                   # in place
+    assert torch.equal(torch.cat(cut(out)), torch.cat(cut(flat)))
+
+
+def test_offsets_past_32_bits(eng):
+    """One tensor of more than 2^31 elements (17 GB): values at its end, at 2^31 elements and at 2^32 bytes."""
+    n = (1 << 31) + 4099
+    if torch.cuda.mem_get_info()[0] < 3 * 8 * n:
+        pytest.skip("not enough free memory")
+    x = torch.zeros(n, dtype=F64, device="cuda")
+    at = torch.tensor([0, (1 << 29) - 1, 1 << 29, (1 << 30) + 1, (1 << 31) - 1, 1 << 31, n - 2, n - 1], device="cuda")
+    x[at] = torch.tensor([1.0, -2.0, 3.0, 4.0, -5.0, 6.0, 7.0, 8.0], dtype=F64, device="cuda")
+    n2 = math.sqrt(204.0)
+    assert G.grad_norms([x]).tolist() == [n2, 8.0]
+    g = x[at].clone()
+    assert G.clip_grads([x], 4.0, INF).tolist() == [n2, 8.0]
+    assert torch.equal(x[at], g * 0.5) and int(torch.count_nonzero(x)) == 8
+    p = torch.zeros_like(x)
+    G.sgd_step([p], [x], lr=2.0)
+    assert torch.equal(p[at], -g) and int(torch.count_nonzero(p)) == 8
+    del x, p
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -328,7 +382,7 @@ def test_refusals(eng):
     import ctypes as C
     e = _native.engine()
     e._bind_dtype(F64)
-    ws = torch.empty(4 * 1026, dtype=F64, device="cuda")
+    ws = torch.empty(4 * 1105, dtype=F64, device="cuda")
     n = (C.c_longlong * 1)(8)
     pt = e._ptrs([t])
     lib, vp = e.lib, C.c_void_p

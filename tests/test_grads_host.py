@@ -215,9 +215,20 @@ def test_which_lists_go_the_short_way():
 def test_the_workspace_is_what_the_header_asks_for():
     from conftest import REPO
     src = open(os.path.join(REPO, "include", "ctm_hip.h")).read()
-    assert "#define CTM_GRAD_WS_DOUBLES(nt) (4 * (1025 + (nt)))" in src
+    assert "#define CTM_GRAD_WS_DOUBLES(nt) (4 * (1089 + 16 * (nt)))" in src
     for nt in (0, 1, 300):
-        assert HostEngine()._grad_ws(nt).numel() == 4 * (1025 + nt)
+        assert HostEngine()._grad_ws(nt).numel() == 4 * (1089 + 16 * nt)
+
+
+def test_tables_and_overlaps_of_lists(tmp_path):
+    """csrc/grads_lists.h compiled by itself (lists_check.cpp): what the launches carry, and which calls are refused."""
+    import subprocess
+    from conftest import PKG, REPO
+    exe = str(tmp_path / "lists_check")
+    subprocess.run(["g++", "-O1", "-g", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I", os.path.join(PKG, "csrc"), os.path.join(REPO, "tests", "lists_check.cpp"),
+                    "-o", exe], check=True, timeout=120)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout == "ok\n", (r.stdout, r.stderr[-2000:])
 
 
 def test_optimizer_refusals():
