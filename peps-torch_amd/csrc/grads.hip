@@ -204,24 +204,32 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const Part* part, int
     if (threadIdx.x == 0) put_norms(r, ws);
 }
 
-// Where the second pass gets its factor from: every workgroup joins the partial results by itself (32 kB from the L2 cache; all get the same bits),
-// which is as fast as a kernel in between on long lists and saves its 4 us on short ones.
+// Where the second pass gets its factor from.  Lists of at most LONG chunks: every workgroup joins the partial results by itself (all get the same
+// bits) while its part of the list is on its way, which saves the 4 us of a kernel in between.  Longer ones, of many times more workgroups
+// than partial results: from ws, where norm_finish_kernel left it (np = 0).
 struct Source { const Part* part; int np; Bound bd; double* ws; bool write; };      // write: one workgroup leaves the norms in ws
 __device__ __forceinline__ double factor(const Source& s) {
     if (s.bd.max_norm < 0.0) return 1.0;
+    if (s.np == 0) return s.ws[2];
     const Norms r = join_partials<THREADS>(s.part, s.np, s.bd);
     if (s.write && blockIdx.x == 0 && threadIdx.x == 0) put_norms(r, s.ws);
     return r.c;
 }
 
-// y = c x (p[0] = x, p[1] = y).  A list inside the bound (c = 1) is left untouched in place.
+// y = c x (p[0] = x, p[1] = y).  In place a list inside the bound (c = 1) is neither read nor written.
 template <bool NT>
 __global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const Source s) {
-    const double c = factor(s);
+    double c = 0.0;
+    bool known = false;
     chunks<2>(t, [&](double* const* p, long long a, long long n) {
-        if (c == 1.0 && p[0] == p[1]) return;
         d2 v[UNROLL];
-        load_chunk<false>(v, p[0], a, n);
+        const bool apart = p[0] != p[1];
+        if (apart) load_chunk<false>(v, p[0], a, n);
+        if (!known) { c = factor(s); known = true; }
+        if (!apart) {
+            if (c == 1.0) return;
+            load_chunk<false>(v, p[0], a, n);
+        }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) v[u] *= c;
         store_chunk<NT>(v, p[1], a, n);
@@ -240,12 +248,14 @@ template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d,
 // p[0] = parameters, p[1] = gradients, p[2] = momentum buffers (MOMENTUM)
 template <bool MOMENTUM, bool NT>
 __global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 : 2> t, const Step s, const Source src) {
-    const double c = factor(src);
+    double c = 0.0;
+    bool known = false;
     chunks<MOMENTUM ? 3 : 2>(t, [&](double* const* p, long long a, long long n) {
         d2 x[UNROLL], d[UNROLL], m[UNROLL];
         load_chunk<false>(d, p[1], a, n);
         if (MOMENTUM && !s.first) load_chunk<false>(m, p[MOMENTUM ? 2 : 0], a, n);
         load_chunk<false>(x, p[0], a, n);
+        if (!known) { c = factor(src); known = true; }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) step_pair<MOMENTUM>(x[u], d[u], m[u], c, s);
         if (MOMENTUM) store_chunk<NT>(d, p[MOMENTUM ? 2 : 0], a, n);
@@ -357,8 +367,10 @@ template <int OP> bool small(ctm_ctx* ctx, hipStream_t s, const Lists<Shape<OP>:
 // than the 32 MB of L2 cache bypass it (545 MB scaled in 185 us against 188 ... 229).
 constexpr long long LLC_BYTES = 256LL << 20, L2_BYTES = 32LL << 20;
 
-// The norm pass; the partial results are at ws + WS_HEAD
-int norm_pass(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, double* ws, int* count) {
+constexpr unsigned LONG = 8192;        // (4752 chunks clipped: 42.3 us joined by the workgroups, 43.7 with the kernel; 66560: 542 and 533)
+
+// The norm pass, and where a second pass finds the factor (`last`: there is none, the norms are to be in ws)
+int norm_pass(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, Bound bd, bool last, double* ws, Source* src) {
     Part* part = (Part*)(ws + WS_HEAD);
     int np = 0;
     for (int i = 0; i < L.nt;) {
@@ -378,12 +390,14 @@ int norm_pass(ctm_ctx* ctx, hipStream_t s, const Lists<1>& L, const Size& z, dou
         }
         np += (int)grid;
     }
-    *count = np;
+    const bool finish = last || z.chunks > LONG;
+    if (finish) GRADS_LAUNCH(ctx, s, norm_finish_kernel, 1, 1024, (const Part*)part, np, bd, ws);
+    *src = Source{part, finish ? 0 : np, bd, ws, !finish};
     return CTM_OK;
 }
 
-// Second pass over a list: launch(table, workgroups, source) for every table of it.  One workgroup per chunk: the table's lookup and the joining of
-// the partial results cost less than the tail of a grid that walks (1.1 GB clipped: 535 us against 553 with 8192 workgroups, 569 with 2048).
+// Second pass over a list: launch(table, workgroups, source) for every table of it.  One workgroup per chunk: the table's lookup costs
+// less than the tail of a grid that walks (1.1 GB clipped: 535 us against 553 with 8192 workgroups, 569 with 2048).
 constexpr unsigned MOST = 1u << 23;          // (a grid holds at most 2^32 threads)
 template <int NP, class F> int second_pass(const Lists<NP>& L, Source src, F&& launch) {
     for (int i = 0; i < L.nt;) {
@@ -421,10 +435,8 @@ int ctm_grad_norms(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* 
     const Bound none{-1.0, 0};
     int status;
     if (small<OP_NORMS>(ctx, s, L, z, none, Step{}, ws, &status)) return status;
-    int np;
-    CTM_TRY(norm_pass(ctx, s, L, z, ws, &np));
-    GRADS_LAUNCH(ctx, s, norm_finish_kernel, 1, 1024, (const Part*)(ws + WS_HEAD), np, none, ws);
-    return CTM_OK;
+    Source src;
+    return norm_pass(ctx, s, L, z, none, true, ws, &src);
     });
 }
 
@@ -442,9 +454,9 @@ int ctm_grad_clip(ctm_ctx* ctx, void* hip_stream, int nt, const double* const* x
     const Bound bd{max_norm, norm_type == CTM_NORM_INF};
     const Size z = size_of(n, nt, L.unit);
     int status;
-    Source src{(const Part*)(ws + WS_HEAD), 0, bd, ws, true};
+    Source src;
     if (small<OP_CLIP>(ctx, s, L, z, bd, Step{}, ws, &status)) return status;
-    CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, ws, &src.np));
+    CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {x}, n, L.unit}, z, bd, false, ws, &src));
     return second_pass(L, src, [&](const Table<2>& t, unsigned grid, const Source& f) -> int {
         if (z.bytes > L2_BYTES) GRADS_LAUNCH(ctx, s, clip_kernel<true>, grid, THREADS, t, f);
         else GRADS_LAUNCH(ctx, s, clip_kernel<false>, grid, THREADS, t, f);
@@ -472,11 +484,11 @@ int ctm_sgd_step(ctm_ctx* ctx, void* hip_stream, int nt, double* const* p, const
     const Step st{lr, momentum, 1.0 - dampening, first};
     const Size z = size_of(n, nt, L2.unit);
     const Bound bd{bounded ? max_norm : -1.0, norm_type == CTM_NORM_INF};
-    Source src{(const Part*)(ws + WS_HEAD), 0, bd, ws, true};          // (no bound: none of it is read)
+    Source src{nullptr, 0, bd, ws, false};
     if (bounded) {
         int status;
         if (m ? small<OP_SGD_MOMENTUM>(ctx, s, L3, z, bd, st, ws, &status) : small<OP_SGD>(ctx, s, L2, z, bd, st, ws, &status)) return status;
-        CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {g}, n, L2.unit}, z, ws, &src.np));
+        CTM_TRY(norm_pass(ctx, s, Lists<1>{nt, {g}, n, L2.unit}, z, bd, false, ws, &src));
     }
     return m ? sgd<true>(ctx, s, L3, z, st, src) : sgd<false>(ctx, s, L2, z, st, src);
     });

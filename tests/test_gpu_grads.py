@@ -147,11 +147,12 @@ def test_step_of_lists(eng, name, dtype, mu, tau, first, max_ratio):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_lists_longer_than_the_caches(eng, dtype):
-    """Whole numbers and factors of 1/2, so that every product and sum is exact: the results equal torch's bit for bit.  0.37 GB, of odd lengths at
-    odd places."""
+@pytest.mark.parametrize("scale", [1, 8])
+def test_lists_longer_than_the_caches(eng, dtype, scale):
+    """Whole numbers and factors of 1/2, so that every product and sum is exact: the results equal torch's bit for bit.  0.37 GB and 46 MB, of odd
+    lengths at odd places."""
     u = 2 if dtype == C128 else 1
-    lens = [35000003 // u, 5, 9000001 // u, 2048, 2300001 // u]
+    lens = [35000003 // u // scale, 5, 9000001 // u // scale, 2048, 2300001 // u // scale]
     flat = torch.randint(-3, 4, (sum(lens) + 7, u), device="cuda", generator=torch.Generator("cuda").manual_seed(11)).to(F64)
     flat = torch.view_as_complex(flat) if u == 2 else flat[:, 0]
     cut = lambda t: list(t[1:1 + sum(lens)].split(lens))              # noqa: E731
@@ -176,6 +177,9 @@ def test_lists_longer_than_the_caches(eng, dtype):
     wp = p - 0.25 * flat
     wp[:1], wp[1 + sum(lens):] = p[:1], p[1 + sum(lens):]
     assert torch.equal(q, wp)
+    keep = flat.clone()
+    G.clip_grads(cut(flat), n2 * 2)                                   # inside the bound
+    assert torch.equal(flat, keep)
     G.clip_grads(cut(flat), n2 / 2)                                   # in place
     assert torch.equal(torch.cat(cut(out)), torch.cat(cut(flat)))
 
