@@ -567,3 +567,32 @@ def test_bounded_gradients_of_lbfgs_on_the_engine(eng, tmp_path):
     c = 1e-3 / n
     t = min(1.0, 1.0 / float((c * g).abs().sum())) * 0.5              # torch's first step of L-BFGS
     assert abs(tight[1][0][0] / n - 1) < 1e-13 and float((tight[2] - (tight[3] - t * c * g)).abs().max()) < 1e-13
+
+
+@pytest.mark.parametrize("script,extra", [("optim_j1j2_c4v.py", ["--optimizer", "sgd", "--OPTARGS_momentum", "0.5"]),
+                                          ("optim_j1j2.py", ["--optimizer", "sgd", "--tiling", "BIPARTITE"]),
+                                          ("optim_j1j2_c4v.py", ["--GLOBALARGS_dtype", "complex128"])])
+def test_optimisation_commands(tmp_path, script, extra):
+    """The commands with gradient descent and with bounded gradients: they run their epochs, log the norms of the gradients and leave state and
+    checkpoint behind; a momentum step is no longer than lr times the bound over 1 - momentum."""
+    import json, os, subprocess, sys
+    from conftest import PKG
+    env = dict(os.environ, PYTHONPATH=PKG + os.pathsep + os.environ.get("PYTHONPATH", ""))
+    pre = str(tmp_path / "o")
+    lr, bound = 0.05, 0.01
+    args = [sys.executable, os.path.join(PKG, "examples", "j1j2", script), "--bond_dim", "2", "--chi", "8", "--opt_max_iter", "3", "--seed", "123",
+            "--CTMARGS_ctm_max_iter", "6", "--GLOBALARGS_device", "cuda:0", "--out_prefix", pre, "--OPTARGS_lr", str(lr), "--OPTARGS_clip_grad_norm", str(bound)]
+    r = subprocess.run(args + extra, capture_output=True, text=True, env=env, timeout=110)
+    assert r.returncode == 0, r.stderr[-3000:]
+    lines = [json.loads(l[l.index("{"):]) for l in open(pre + ".log") if "grad_mag" in l]
+    assert len(lines) == 3 and all(l["grad_mag"][0] >= l["grad_mag"][1] > 0 for l in lines)
+    assert os.path.exists(pre + "_state.json")
+    ck = torch.load(pre + "_checkpoint.p", weights_only=False, map_location="cpu")
+    group = ck["optimizer_state_dict"]["param_groups"][0]
+    if "sgd" in extra:
+        assert group["lr"] == lr and group["max_norm"] == bound
+        if "--OPTARGS_momentum" in extra:
+            m = torch.cat([s["momentum_buffer"].reshape(-1) for s in ck["optimizer_state_dict"]["state"].values()])
+            assert float(torch.linalg.vector_norm(m)) <= bound / (1 - 0.5) * (1 + 1e-12)
+    else:
+        assert "history_size" in group
