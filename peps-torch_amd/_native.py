@@ -179,7 +179,7 @@ def _is_dense(t):
 
 
 def _sequence(x):
-    return x if type(x) in (list, tuple) else list(x)
+    return x if type(x) in (list, tuple) else [x] if isinstance(x, torch.Tensor) else list(x)
 
 
 def _put_back(pairs):
@@ -965,12 +965,12 @@ class Engine:
                 raise NativeError(f"{what}: {name} {i} is {tuple(y.shape)} {y.dtype}, its tensor {tuple(x.shape)} {x.dtype}")
 
     @staticmethod
-    def _written(what, outs):
-        """Tensors that a call writes: memory of their own, every element of its own, holding the values themselves.  (The library compares the
-        ranges of contiguous tensors; here the extents, where one of the tensors is a strided view.)"""
+    def _written(what, outs, lazy=False):
+        """Tensors that a call writes: memory of their own, every element of its own, holding the values themselves unless `lazy`.  (The library
+        compares the ranges of contiguous tensors; here the extents, where one of the tensors is a strided view.)"""
         views = False
         for i, t in enumerate(outs):
-            if t.is_conj() or t.is_neg():
+            if not lazy and (t.is_conj() or t.is_neg()):
                 raise NativeError(f"{what}: tensor {i} is a lazily conjugated or negated view: it cannot be written")
             if not t.is_contiguous():
                 views = True
@@ -1048,7 +1048,7 @@ class Engine:
         else:
             outs, _ = self._list(what, out)
             self._same_lists(what, ts, outs, "outputs")
-        self._written(what, outs)
+        self._written(what, outs, lazy=out is None)          # (a real factor commutes with a pending conjugation or sign: autograd leaves such gradients)
         xs, ys, back = [], [], []
         for i, (x, y) in enumerate(zip(ts, outs)):
             if not (x is y and _is_dense(x)):

@@ -10,7 +10,9 @@ without limit next to degenerate singular values (linalg/svd_gesdd.py:209-328 re
 
 All tensors of a list are on one device and of one dtype; empty tensors, 0-dimensional tensors, strided views and empty lists are allowed.  A NaN
 anywhere makes both norms NaN and a clipped list all NaN; an infinite element makes c = 0 (0 x inf = NaN).  Calls run on the current stream, do not
-synchronise and may be captured into a graph (after one call outside of it, which makes the native context); they are not differentiable."""
+synchronise and may be captured into a graph (after one call outside of it, which makes the native context); they are not
+differentiable.  As every call of an engine they are one thread's at a time: another thread inside the same engine makes them raise NativeError."""
+import torch
 from backend import get_engine
 
 
@@ -26,7 +28,9 @@ def clip_grads(tensors, max_norm, norm_type=2, out=None):
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2):
-    """clip_grads, in place, of the `.grad` of a list of parameters (those without one are left out)."""
+    """clip_grads, in place, of the `.grad` of a list of parameters (those without one are left out) or of one parameter."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
     return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm, norm_type=norm_type)
 
 

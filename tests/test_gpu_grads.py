@@ -76,7 +76,7 @@ LISTS = {
     "chunks": [4095, 4096, 8191, 8193],
     "empties_between": [0, 5, 0, 0, 513, 0], "pieces": [127, 128, 129, 255], "one_group": [16384], "one_group_half": [8192], "one_group_quarter": [4096],
     "group_of_many": [256] * 63 + [255], "group_and_one": [16383, 1], "over_group": [16385], "cell_D4": [512] * 4, "cell_D8": [8192] * 8,
-    "table_full": [3] * 64, "table_over": [5] * 65, "many": [(37 * i) % 411 for i in range(300)], "long": [1 << 19, 3, 277777],
+    "short_ones": [3] * 64, "table_full": [5] * 192 + [0] * 7, "table_over": [7] * 257, "several_tables": [(13 * i) % 97 + 1 for i in range(700)] + [30001], "many": [(37 * i) % 411 for i in range(300)], "long": [1 << 19, 3, 277777],
     "one_long": [1500001],
 }
 
@@ -276,6 +276,9 @@ def test_orders_and_strides(eng, dtype):
             check_norms(G.grad_norms([v]), [np.ascontiguousarray(a)])
             o = torch.empty(v.shape, dtype=v.dtype, device="cuda")
             G.clip_grads([v], 0.25, out=[o])
+            w = v.clone()                                             # (keeps the flag of a conjugate)
+            G.clip_grads([w], 0.25)
+            check_clip(host([w]), [np.ascontiguousarray(a)], 0.25, 2, O.norms([np.ascontiguousarray(a)]))
             check_clip(host([o]), [np.ascontiguousarray(a)], 0.25, 2, O.norms([np.ascontiguousarray(a)]))
 
 
@@ -372,7 +375,7 @@ def test_refusals(eng):
            lambda: G.grad_norms([t.to_sparse()]), lambda: G.clip_grads([t], -1.0), lambda: G.clip_grads([t], float("nan")),
            lambda: G.clip_grads([t], 1.0, norm_type=1), lambda: G.clip_grads([t], 1.0, out=[]), lambda: G.clip_grads([t], 1.0, out=[u[:7]]),
            lambda: G.clip_grads([t, t], 0.5), lambda: G.clip_grads([t[:5], t[4:]], 0.5), lambda: G.clip_grads([t, u], 0.5, out=[u, t]),
-           lambda: G.clip_grads([t[:4]], 0.5, out=[t[2:6]]), lambda: G.clip_grads([t[:1].expand(3)], 0.5), lambda: G.clip_grads([z.conj()], 0.5),
+           lambda: G.clip_grads([t[:4]], 0.5, out=[t[2:6]]), lambda: G.clip_grads([t[:1].expand(3)], 0.5), lambda: G.clip_grads([z], 0.5, out=[torch.ones_like(z).conj()]),
            lambda: G.clip_grads([t[0:6:2], t[1:7:2]], 0.5),
            lambda: G.sgd_step([t], [u], lr=-1.0), lambda: G.sgd_step([t], [u], momentum=0.5), lambda: G.sgd_step([t], [u, u]),
            lambda: G.sgd_step([t], [t]), lambda: G.sgd_step([t], [u], [t], momentum=0.5), lambda: G.sgd_step([t], [u], [u], momentum=0.5),

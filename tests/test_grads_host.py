@@ -156,13 +156,39 @@ def test_conjugated_negated_and_broadcast_inputs(host):
     assert torch.equal(p, -z.conj())
 
 
+def test_gradients_with_a_pending_conjugation_or_sign(host):
+    """What autograd leaves in `.grad`: scaled in place, whatever the flag says about the memory."""
+    z = t64(3, 4, dtype=torch.complex128)
+    n = float(torch.linalg.vector_norm(z))
+    for view in (lambda t: t.conj(), lambda t: t.conj().t(), lambda t: t.conj()[1:, ::2]):
+        m = z.clone()
+        v = view(m)
+        k = float(torch.linalg.vector_norm(v))
+        got = G.clip_grads([v], 0.25)
+        want = z.clone()
+        view(want).mul_(0.25 / k)
+        assert abs(float(got[0]) / k - 1) < 1e-14 and torch.allclose(m, want, rtol=1e-14, atol=0) and v.is_conj()
+    m = z.clone()
+    G.clip_grads([m.conj().imag], 0.0)
+    assert torch.equal(m, torch.complex(z.real, torch.zeros_like(z.real)))
+    p = torch.zeros_like(z).requires_grad_()
+    p.grad = z.clone().conj()
+    assert p.grad.is_conj()
+    G.clip_grad_norm_([p], 1.0)
+    assert torch.allclose(p.grad, z.conj() / n, rtol=1e-14, atol=0)
+    G.clip_grad_norm_(p, 0.5)
+    assert torch.allclose(p.grad, z.conj() * (0.5 / n), rtol=1e-14, atol=0)
+    assert torch.equal(G.grad_norms(z), G.grad_norms([z]))
+
+
 def test_refusals_before_anything_is_written(host):
     t, u, z = torch.ones(8, dtype=torch.float64), torch.ones(8, dtype=torch.float64), torch.ones(8, dtype=torch.complex128)
     meta = torch.ones(8, dtype=torch.float64, device="meta")
     bad = [lambda: G.grad_norms([t, meta]), lambda: G.grad_norms([t.float()]), lambda: G.grad_norms([t, z]), lambda: G.grad_norms([t, None]),
            lambda: G.grad_norms([3.0]), lambda: G.grad_norms([t.to_sparse()]), lambda: G.clip_grads([t], -1.0), lambda: G.clip_grads([t], float("nan")),
            lambda: G.clip_grads([t], 1.0, norm_type=1), lambda: G.clip_grads([t], 1.0, out=[]), lambda: G.clip_grads([t], 1.0, out=[u[:7]]),
-           lambda: G.clip_grads([t[:1].expand(3)], 0.5), lambda: G.clip_grads([z.conj()], 0.5), lambda: G.clip_grads([t[0:6:2], t[1:7:2]], 0.5),
+           lambda: G.clip_grads([t[:1].expand(3)], 0.5), lambda: G.clip_grads([z], 0.5, out=[torch.ones_like(z).conj()]),
+           lambda: G.sgd_step([z.conj()], [torch.ones_like(z)], lr=0.5), lambda: G.clip_grads([t[0:6:2], t[1:7:2]], 0.5),
            lambda: G.clip_grads([t.as_strided((3, 3), (2, 1))], 0.5), lambda: G.clip_grads([t[::2], t[:4]], 0.5),
            lambda: G.sgd_step([t], [u], lr=-1.0), lambda: G.sgd_step([t], [u], momentum=0.5), lambda: G.sgd_step([t], [u, u]),
            lambda: G.sgd_step([t], [u], [u[:4]], momentum=0.5), lambda: G.sgd_step([t[::2]], [u[::2]], [t[::2]], momentum=0.5),
