@@ -109,8 +109,9 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
     """Minimise `loss_fn(state, env, opt_context) -> (loss, env, history, t_ctm, t_obs[, t_loss])` over the on-site tensors of
     `state`.  Every evaluation starts from the environment the previous one returned (detached); the lowest-loss state is written
     to `<out_prefix>_state.json`, a checkpoint before every step to `<out_prefix>_checkpoint.p`.  `create` / `load` make and restore the
-    optimiser (ad_optim_sgd_mod: gradient descent).  `opt_args.clip_grad_norm` > 0 bounds the 2-norm of the gradient that reaches it; the log
-    and the `tolerance_grad` test see the gradient itself."""
+    optimiser (ad_optim_sgd_mod: gradient descent).  `opt_args.clip_grad_norm` > 0 bounds the 2-norm of the gradient that an epoch steps along:
+    gradient descent scales it inside its step, L-BFGS makes the step of the scaled gradient with the curvature of the gradient itself
+    (bounded_step), any other optimiser gets it scaled.  The log and all tolerances mean the gradient itself."""
     verbosity = opt_args.verbosity_opt_epoch
     checkpoint_file = main_args.out_prefix + "_checkpoint.p"
     outputstatefile = main_args.out_prefix + "_state.json"
@@ -122,8 +123,11 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
     if main_args.opt_resume is not None:
         load(optimizer, state, main_args=main_args, opt_args=opt_args, ctm_args=ctm_args, global_args=global_args)
     calls = [0]
-    clip = opt_args.clip_grad_norm if isinstance(optimizer, torch.optim.LBFGS) else 0.0        # (gradient descent scales inside its step)
-    raw_norms = [None]                                                                         # of the last gradient, where it was scaled in place
+    bounded_lbfgs = opt_args.clip_grad_norm > 0.0 and isinstance(optimizer, torch.optim.LBFGS)
+    clip = 0.0 if bounded_lbfgs or "max_norm" in optimizer.param_groups[0] else opt_args.clip_grad_norm
+    if bounded_lbfgs and (optimizer.param_groups[0].get("line_search_fn") is not None or opt_args.line_search == "backtracking"):
+        raise RuntimeError("clip_grad_norm needs the fixed step (line_search default)")        # (a checkpoint brings its line search along)
+    raw_norms = [None]                                          # of the last gradient, where it was scaled in place
 
     def _write_best():
         if parallel.world()[0] == 0:        # replicated run: one writer
@@ -190,6 +194,49 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
             obs_fn(state, current_env[0], context)
         return loss.item()
 
+    def move(x0, d, alpha):
+        """parameters <- x0 + alpha d, d as torch's optimiser lays it out."""
+        off = 0
+        with torch.no_grad():
+            for p, x in zip(parameters, x0):
+                n = p.numel() * (2 if p.is_complex() else 1)
+                step = d[off:off + n]
+                step = torch.view_as_complex(step.view(-1, 2)).view_as(p) if p.is_complex() else step.view_as(p)
+                p.copy_(x + alpha * step)
+                off += n
+
+    def bounded_step():
+        """An epoch of L-BFGS under `clip_grad_norm`.  Direction, history and tolerances are those of the gradient itself (differences of gradients
+        that were scaled by different factors are no curvature, and what is left of a scaled gradient says nothing about convergence); the step is
+        the one that this history makes of the scaled gradient c g: c times as long, the first one lr c min(1, 1 / |c g|_1).  It is never
+        longer than without the bound.  The iterations of an epoch are made one by one, since each is shortened before the next
+        evaluation, with the ends that torch's own loop of `max_iter` iterations has."""
+        group, st = optimizer.param_groups[0], optimizer.state[parameters[0]]
+        iters, last = group["max_iter"], None
+        group["max_iter"] = 1
+        try:
+            for it in range(iters):
+                with torch.enable_grad():
+                    loss = closure()
+                value = float(loss.detach())
+                if it > 0 and (it + 1 >= group["max_eval"] or float(st["d"].mul(st["t"]).abs().max()) <= group["tolerance_change"]
+                               or abs(value - last) < group["tolerance_change"]):
+                    break
+                x0, versions = [p.detach().clone() for p in parameters], [p._version for p in parameters]
+                optimizer.step(lambda: loss)
+                if [p._version for p in parameters] == versions:      # it stopped where it was
+                    break
+                n = _grad_norms([p.grad for p in parameters if p.grad is not None and p.grad.numel()])[0]
+                if n > opt_args.clip_grad_norm:
+                    c = opt_args.clip_grad_norm / n
+                    st["t"] = group["lr"] * c
+                    if st["n_iter"] == 1:
+                        st["t"] /= max(1.0, float(st["prev_flat_grad"].mul(c).abs().sum()))
+                    move(x0, st["d"], st["t"])
+                last = value
+        finally:
+            group["max_iter"] = iters
+
     def backtracking_step():
         """One L-BFGS iteration whose step length comes from the derivative-free Armijo search: torch's optimiser computes the
         direction with lr = 1 (its step is undone), the search then moves along it."""
@@ -209,18 +256,8 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
         g = st["prev_flat_grad"]
         gtd = float(torch.real(torch.vdot(g, d))) if g.is_complex() else float(g.dot(d))
 
-        def move(alpha):
-            off = 0
-            with torch.no_grad():
-                for p, x in zip(parameters, x0):
-                    n = p.numel() * (2 if p.is_complex() else 1)
-                    step = d[off:off + n]
-                    step = torch.view_as_complex(step.view(-1, 2)).view_as(p) if p.is_complex() else step.view_as(p)
-                    p.copy_(x + alpha * step)
-                    off += n
-
         def phi(alpha):
-            move(alpha)
+            move(x0, d, alpha)
             return closure_linesearch()
         alpha, _ = _armijo(phi, loss0, gtd, alpha0=float(t))
         while alpha is None and t > opt_args.line_search_tol:
@@ -229,7 +266,7 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
         if alpha is None:
             raise RuntimeError("minimize_scalar failed")
         log.info(f"LS final step: {alpha}")
-        move(alpha)
+        move(x0, d, alpha)
         st["t"] = alpha
         group["lr"] = lr0
 
@@ -239,6 +276,8 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
         calls[0] = 0
         if opt_args.line_search == "backtracking":
             backtracking_step()
+        elif bounded_lbfgs:
+            bounded_step()
         else:
             optimizer.step(closure)
         t_data["loss_ls"] = []

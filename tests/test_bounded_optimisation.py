@@ -1,0 +1,108 @@
+"""CPU: bounded gradients in the optimisation driver over several epochs -- L-BFGS whose gradients are scaled now and then, tolerances that mean the
+gradient itself, epochs of several iterations; what a step that failed leaves behind."""
+import numpy as np
+import pytest
+import torch
+from test_grads_host import host, run, t64  # noqa: F401  (fixture)
+from optim import ad_optim_lbfgs_mod as L
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.complex128])
+@pytest.mark.parametrize("ratio", [0.9, 0.7, 0.5, 0.3, 0.1])
+def test_scaling_that_comes_to_an_end_on_the_way(host, tmp_path, dtype, ratio):
+    """A convex quadratic whose gradient is scaled at the start and no longer later on: the loss never rises and reaches its minimum.  (Its Hessian is
+    the identity: every secant pair of true gradients gives H = 1, so each epoch behind the first moves by 0.5 c g.)"""
+    a0 = t64(2, 2, 2, 2, 2, seed=3, dtype=dtype)
+    n0 = float(torch.linalg.vector_norm(a0 - 1.0))
+    free = run(tmp_path, L, dtype=dtype, lr=0.5, epochs=60, tolerance_grad=0.0)[0]
+    losses, mags, a, _ = run(tmp_path, L, dtype=dtype, lr=0.5, epochs=60, tolerance_grad=0.0, clip_grad_norm=ratio * n0)
+    assert mags[0][0] > ratio * n0 > mags[-1][0]
+    for r in (free, losses):
+        assert all(y < x or y < 1e-24 for x, y in zip(r, r[1:])) and r[-1] < 1e-10 * r[0]
+    # the loss of each epoch behind the second from the one before: g <- (1 - 0.5 c) g
+    for (n, _), (m, _) in list(zip(mags[1:], mags[2:]))[:20]:
+        assert abs(m / n - (1.0 - 0.5 * min(1.0, ratio * n0 / n))) < 1e-9
+
+
+@pytest.mark.parametrize("bound", [1e-3, 1e-5, 5e-6, 1e-9])
+def test_a_bound_below_the_tolerances_still_moves(host, tmp_path, bound):
+    """The tolerances of the optimiser mean the gradient, not what is left of it: elements of the scaled gradient below tolerance_grad, a squared norm
+    below tolerance_change."""
+    losses, mags, a, a0 = run(tmp_path, L, lr=0.5, epochs=4, clip_grad_norm=bound, tolerance_grad=1e-5, tolerance_change=1e-30)
+    n = mags[0][0]
+    assert len(losses) == 4 and all(abs(m[0] / n - 1.0) < 1e-3 for m in mags)
+    # four steps of 0.5 c g, |c g| = bound; values below 4: each step rounds each of the 32 elements by 4 x 2^-53 at most
+    assert abs(float(torch.linalg.vector_norm(a - a0)) / (4 * 0.5 * bound) - 1.0) < 1e-6 + 4 * 32 ** 0.5 * 4 * 2.0 ** -53 / (2 * bound)
+    g = a0 - 1.0
+    assert float((a - (a0 - 4 * 0.5 * bound * g / n)).abs().max()) < 1e-5 * bound + 1e-15
+
+
+def test_the_raw_gradient_ends_the_run(host, tmp_path):
+    """max |g| <= tolerance_grad: nothing moves, whether the gradient would be scaled or not."""
+    for bound in (0.0, 1e-2, 1e2):
+        losses, _, a, a0 = run(tmp_path, L, lr=0.5, epochs=4, clip_grad_norm=bound, tolerance_grad=1e3)
+        assert len(losses) == 1 and torch.equal(a, a0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.complex128])
+@pytest.mark.parametrize("iters", [1, 2, 3, 4, 5, 8])
+@pytest.mark.parametrize("tol", [0.0, 1e-9, 1e-3])
+def test_a_bound_above_the_norm_changes_nothing(host, tmp_path, dtype, iters, tol):
+    """Bit for bit, down to convergence, with several iterations per epoch."""
+    kw = dict(dtype=dtype, lr=0.75, epochs=12, max_iter_per_epoch=iters, tolerance_change=tol, tolerance_grad=1e-7)
+    free, wide = run(tmp_path, L, **kw), run(tmp_path, L, clip_grad_norm=1e6, **kw)
+    assert free[0] == wide[0] and torch.equal(free[2], wide[2]) and np.allclose(free[1], wide[1], rtol=1e-14)
+
+
+def test_several_scaled_iterations_per_epoch(host, tmp_path):
+    """Iterations of one epoch are those of epochs of one iteration."""
+    # (an epoch of 3 iterations of torch's L-BFGS makes 3 evaluations, the last of which ends it: 2 steps)
+    one = run(tmp_path, L, lr=0.5, epochs=2, clip_grad_norm=0.5, tolerance_grad=0.0)
+    many = run(tmp_path, L, lr=0.5, epochs=1, max_iter_per_epoch=3, clip_grad_norm=0.5, tolerance_grad=0.0)
+    assert len(many[0]) == 3 and many[0][:2] == one[0] and torch.equal(one[2], many[2])
+
+
+def test_history_of_true_gradients_in_the_checkpoint(host, tmp_path):
+    """The optimiser's memory holds the gradient itself: a run that resumes without the bound builds on it."""
+    run(tmp_path, L, lr=0.5, epochs=3, clip_grad_norm=0.25, tolerance_grad=0.0)
+    ck = torch.load(str(tmp_path / "o_checkpoint.p"), weights_only=False)
+    st = next(iter(ck["optimizer_state_dict"]["state"].values()))
+    for y, s in zip(st["old_dirs"], st["old_stps"]):
+        assert float((y - s).abs().max()) <= 8 * 4 * 2.0 ** -53                # (identity Hessian; values below 4, a rounding of each operation)
+    assert float(st["prev_flat_grad"].abs().max()) > 0.25
+
+
+def test_a_checkpoint_brings_its_line_search_along(host, tmp_path):
+    """Resumed without override it is the stored search that would run: refused under a bound, as it is at the start."""
+    run(tmp_path, L, epochs=2, line_search="strong_wolfe")
+    ck = str(tmp_path / "o_checkpoint.p")
+    with pytest.raises(RuntimeError, match="clip_grad_norm needs the fixed step"):
+        run(tmp_path, L, epochs=1, resume=ck, clip_grad_norm=0.5)
+    run(tmp_path, L, epochs=1, resume=ck, override=True, clip_grad_norm=0.5)
+
+
+def test_an_infinite_gradient_does_not_move_the_others(host, tmp_path):
+    """c = 0: nothing is divided by the vanished gradient; 0 x inf is NaN, the other elements stay."""
+    class Infinite(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            g = g.clone()
+            g.view(-1)[5] = float("inf")
+            return g
+    a0 = t64(2, 2, 2, 2, 2, seed=3)
+    import copy
+    import os
+    import config as cfg
+    from ipeps.ipeps_c4v import IPEPS_C4V
+    from test_grads_host import Env
+    st, opt_args, main_args = IPEPS_C4V(a0.clone()), copy.deepcopy(cfg.opt_args), copy.deepcopy(cfg.main_args)
+    opt_args.clip_grad_norm, opt_args.lr = 0.5, 0.5
+    main_args.opt_max_iter, main_args.out_prefix = 1, os.path.join(str(tmp_path), "o")
+    L.optimize_state(st, Env(), lambda s, e, c: (0.5 * (Infinite.apply(s.site()) ** 2).sum(), e, [], 0.0, 0.0), main_args=main_args, opt_args=opt_args)
+    a = st.site().detach().view(-1)
+    other = torch.arange(32) != 5
+    assert torch.isnan(a[5]) and torch.equal(a[other], a0.view(-1)[other])
