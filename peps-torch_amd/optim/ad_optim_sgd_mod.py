@@ -39,22 +39,32 @@ class SGD(torch.optim.Optimizer):
         if group["momentum"] == 0.0:
             self.norms = grads.sgd_step(ps, gs, **kw, **bound)
             return loss
-        new = [p for p in ps if "momentum_buffer" not in self.state[p]]
-        for p in new:
-            self.state[p]["momentum_buffer"] = torch.empty_like(p)
-        bufs = [self.state[p]["momentum_buffer"] for p in ps]
+        # (a call that fails leaves no trace: new buffers count from the call on that has filled them)
+        bufs = [self.state.get(p, {}).get("momentum_buffer") for p in ps]
+        new = [i for i, m in enumerate(bufs) if m is None]
+        for i in new:
+            bufs[i] = torch.empty_like(ps[i])
         if len(new) in (0, len(ps)):
-            self.norms = grads.sgd_step(ps, gs, bufs, first=len(new) > 0, **kw, **bound)
-            return loss
-        # some parameters take their first step, the others do not: two calls, the factor is that of all gradients
-        self.norms = None
-        if bound["max_norm"] is not None:
-            scaled = [torch.empty_like(g) for g in gs]
-            self.norms = grads.clip_grads(gs, out=scaled, **bound)
-            gs = scaled
-        for first in (False, True):
-            part = [i for i, p in enumerate(ps) if any(p is q for q in new) == first]
-            grads.sgd_step([ps[i] for i in part], [gs[i] for i in part], [bufs[i] for i in part], first=first, **kw)
+            norms = grads.sgd_step(ps, gs, bufs, first=len(new) > 0, **kw, **bound)
+        else:
+            # some parameters take their first step, the others do not: two calls, the factor is that of all gradients
+            norms = None
+            if bound["max_norm"] is not None:
+                scaled = [torch.empty_like(g) for g in gs]
+                norms = grads.clip_grads(gs, out=scaled, **bound)
+                gs = scaled
+            before = [ps[i].clone() for i in new]
+            grads.sgd_step([ps[i] for i in new], [gs[i] for i in new], [bufs[i] for i in new], first=True, **kw)
+            rest = [i for i in range(len(ps)) if i not in new]
+            try:
+                grads.sgd_step([ps[i] for i in rest], [gs[i] for i in rest], [bufs[i] for i in rest], **kw)
+            except BaseException:
+                for i, x in zip(new, before):
+                    ps[i].copy_(x)
+                raise
+        for i in new:
+            self.state[ps[i]]["momentum_buffer"] = bufs[i]
+        self.norms = norms
         return loss
 
 

@@ -106,3 +106,85 @@ def test_an_infinite_gradient_does_not_move_the_others(host, tmp_path):
     a = st.site().detach().view(-1)
     other = torch.arange(32) != 5
     assert torch.isnan(a[5]) and torch.equal(a[other], a0.view(-1)[other])
+
+
+# ---- the momentum step that fails -----------------------------------------------------------------------------------------------------------
+
+class Fails:
+    """The host's double of the library with calls that are refused as busy."""
+
+    def __init__(self, host, calls):
+        self.host, self.calls, self.n = host, set(calls), 0
+        self.inner = host.lib.ctm_sgd_step
+        host.lib.ctm_sgd_step = self
+        host.lib.ctm_last_error = lambda h: b"in use"
+        host._bind_dtype = lambda dt: setattr(host._tls, "h", None)
+        import threading
+        host._tls = threading.local()
+        host._tls.h = None
+
+    def __call__(self, *a):
+        self.n += 1
+        return 7 if self.n in self.calls else self.inner(*a)
+
+
+def params(n=3):
+    ps = [t64(4, 3, seed=i).requires_grad_() for i in range(n)]
+    for i, p in enumerate(ps):
+        p.grad = t64(4, 3, seed=10 + i)
+    return ps
+
+
+def garbage(monkeypatch):
+    """Uninitialised memory holds NaN."""
+    empty_like = torch.empty_like
+    monkeypatch.setattr(torch, "empty_like", lambda t, **kw: empty_like(t, **kw).fill_(float("nan")))
+
+
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_a_refused_first_step_leaves_nothing_behind(host, monkeypatch, max_norm):
+    from _native import NativeError
+    from optim.ad_optim_sgd_mod import SGD
+    garbage(monkeypatch)
+    kw = dict(lr=0.25, momentum=0.5, dampening=0.25, max_norm=max_norm)
+    ref, ps = params(), params()
+    a, b = SGD(ref, **kw), SGD(ps, **kw)
+    a.step()
+    a.step()
+    Fails(host, [1])
+    start = [p.detach().clone() for p in ps]
+    with pytest.raises(NativeError, match="busy"):
+        b.step()
+    assert len(b.state_dict()["state"]) == 0 and b.norms is None and all(torch.equal(x, p) for x, p in zip(start, ps))
+    b.step()
+    b.step()
+    assert all(torch.equal(x, y) and torch.equal(a.state[x]["momentum_buffer"], b.state[y]["momentum_buffer"]) for x, y in zip(ref, ps))
+
+
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+@pytest.mark.parametrize("call", [1, 2])
+def test_a_refused_step_of_parameters_that_join_later(host, monkeypatch, call, max_norm):
+    """Either of the two calls of such a step fails: as before the step, and the same step afterwards as without the failure."""
+    from _native import NativeError
+    from optim.ad_optim_sgd_mod import SGD
+    garbage(monkeypatch)
+    kw = dict(lr=0.25, momentum=0.5, dampening=0.25, max_norm=max_norm)
+
+    def one():
+        ps = params()
+        late, ps[1].grad = ps[1].grad, None
+        opt = SGD(ps, **kw)
+        opt.step()
+        ps[1].grad = late
+        return ps, opt
+    ref, a = one()
+    a.step()
+    ps, b = one()
+    start, bufs = [p.detach().clone() for p in ps], [b.state[ps[i]]["momentum_buffer"].clone() for i in (0, 2)]
+    Fails(host, [call])
+    with pytest.raises(NativeError, match="busy"):
+        b.step()
+    assert all(torch.equal(x, p) for x, p in zip(start, ps)) and "momentum_buffer" not in b.state.get(ps[1], {})
+    assert all(torch.equal(x, b.state[ps[i]]["momentum_buffer"]) for x, i in zip(bufs, (0, 2)))
+    b.step()
+    assert all(torch.equal(x, y) and torch.equal(a.state[x]["momentum_buffer"], b.state[y]["momentum_buffer"]) for x, y in zip(ref, ps))
