@@ -25,6 +25,16 @@ class SGD(torch.optim.Optimizer):
         if len(self.param_groups) != 1:
             raise ValueError("SGD: one parameter group only (the norm is that of all parameters)")
 
+    def load_state_dict(self, state_dict):
+        """Of this class or of torch.optim.SGD, which has no bound; what it has besides (weight_decay, nesterov, maximize) is refused."""
+        groups = []
+        for g in state_dict["param_groups"]:
+            for k in ("weight_decay", "nesterov", "maximize"):
+                if g.get(k):
+                    raise ValueError(f"SGD: {k} {g[k]} of the stored state")
+            groups.append({"max_norm": None, "norm_type": 2, **g})
+        super().load_state_dict({**state_dict, "param_groups": groups})
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -82,14 +92,15 @@ def create_optimizer(state, main_args=cfg.main_args, opt_args=cfg.opt_args, ctm_
 
 def load_optimizer_state_(optimizer, state, main_args=cfg.main_args, opt_args=cfg.opt_args, ctm_args=cfg.ctm_args,
                           global_args=cfg.global_args):
-    """Resume from `main_args.opt_resume`; with `opt_resume_override_params` the stored lr, momentum, dampening and bound are replaced by the
-    current OPTARGS."""
+    """Resume from `main_args.opt_resume`, a checkpoint of this optimiser or of torch.optim.SGD (whose bound is that of the current OPTARGS); with
+    `opt_resume_override_params` the stored lr, momentum, dampening and bound are replaced by the current OPTARGS."""
     print(f"INFO: resuming from check point. resume = {main_args.opt_resume}")
     checkpoint = torch.load(main_args.opt_resume, map_location=state.device, weights_only=False)
     sd = checkpoint["optimizer_state_dict"]
     group = sd["param_groups"][0]
     if "dampening" not in group:
         raise RuntimeError(f"{main_args.opt_resume} is not a checkpoint of gradient descent")
+    group.setdefault("max_norm", optimizer.param_groups[0]["max_norm"])          # (a checkpoint of torch.optim.SGD)
     if main_args.opt_resume_override_params:
         group.update(lr=opt_args.lr, momentum=opt_args.momentum, dampening=opt_args.dampening,
                      max_norm=opt_args.clip_grad_norm if opt_args.clip_grad_norm > 0.0 else None)

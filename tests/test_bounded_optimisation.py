@@ -1,5 +1,6 @@
 """CPU: bounded gradients in the optimisation driver over several epochs -- L-BFGS whose gradients are scaled now and then, tolerances that mean the
 gradient itself, epochs of several iterations; what a step that failed leaves behind."""
+import copy
 import numpy as np
 import pytest
 import torch
@@ -94,7 +95,6 @@ def test_an_infinite_gradient_does_not_move_the_others(host, tmp_path):
             g.view(-1)[5] = float("inf")
             return g
     a0 = t64(2, 2, 2, 2, 2, seed=3)
-    import copy
     import os
     import config as cfg
     from ipeps.ipeps_c4v import IPEPS_C4V
@@ -188,3 +188,60 @@ def test_a_refused_step_of_parameters_that_join_later(host, monkeypatch, call, m
     assert all(torch.equal(x, b.state[ps[i]]["momentum_buffer"]) for x, i in zip(bufs, (0, 2)))
     b.step()
     assert all(torch.equal(x, y) and torch.equal(a.state[x]["momentum_buffer"], b.state[y]["momentum_buffer"]) for x, y in zip(ref, ps))
+
+
+# ---- checkpoints of torch's own gradient descent --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("momentum", [0.0, 0.5])
+def test_state_of_torch_sgd_is_taken(host, momentum):
+    """lr, momentum and dampening of torch.optim.SGD and its buffers; it knows no bound.  Without momentum its buffers are None."""
+    from optim.ad_optim_sgd_mod import SGD
+    ref, ps = params(), params()
+    a = torch.optim.SGD(ref, lr=0.25, momentum=momentum, dampening=0.25 if momentum else 0.0)
+    a.step()
+    with torch.no_grad():
+        for x, y in zip(ref, ps):
+            y.copy_(x)
+    b = SGD(ps, lr=1.0, momentum=0.125, max_norm=1e-3)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))          # (torch hands the buffers themselves over: both would write them)
+    for _ in range(2):
+        a.step()
+        b.step()
+    # (values below 4, five roundings a step at most, two steps)
+    assert all(float((x - y).detach().abs().max()) <= 10 * 4 * 2.0 ** -53 for x, y in zip(ref, ps)) and b.norms is None
+    # a momentum that begins later: its first step
+    b.param_groups[0].update(momentum=0.5, dampening=0.0)
+    if momentum == 0.0:
+        before = [p.detach().clone() for p in ps]
+        b.step()
+        assert all(float((x - 0.25 * p.grad - p.detach()).abs().max()) <= 4 * 4 * 2.0 ** -53 for x, p in zip(before, ps))
+
+
+@pytest.mark.parametrize("key,value", [("nesterov", True), ("weight_decay", 0.1), ("maximize", True)])
+def test_state_of_torch_sgd_with_more_than_this_one_has(key, value):
+    """An iteration that this optimiser does not make is refused, not replaced by another."""
+    from optim.ad_optim_sgd_mod import SGD
+    a, b = torch.optim.SGD(params(), lr=0.25, momentum=0.5, **{key: value}), SGD(params(), lr=0.25, momentum=0.5)
+    with pytest.raises(ValueError, match=key):
+        b.load_state_dict(a.state_dict())
+    assert "nesterov" not in b.param_groups[0]
+
+
+@pytest.mark.parametrize("override", [False, True])
+def test_a_run_resumes_from_a_checkpoint_of_torch_sgd(host, tmp_path, override):
+    """The bound, which the checkpoint does not have, is that of the run."""
+    import os
+    from optim import ad_optim_sgd_mod as S
+    a0 = t64(2, 2, 2, 2, 2, seed=3)
+    p = a0.clone().requires_grad_()
+    opt = torch.optim.SGD([p], lr=0.25, momentum=0.5)
+    p.grad = t64(2, 2, 2, 2, 2, seed=4)
+    opt.step()
+    m = opt.state[p]["momentum_buffer"].clone()
+    ck = os.path.join(str(tmp_path), "torch.p")
+    torch.save({"epoch": 1, "loss": 0.0, "parameters": {}, "optimizer_state_dict": opt.state_dict()}, ck)
+    _, _, a, _ = run(tmp_path, S, epochs=1, resume=ck, override=override, lr=0.125, momentum=0.75, tolerance_grad=0.0, clip_grad_norm=0.5)
+    g = a0 - 1.0
+    lr, mu = (0.125, 0.75) if override else (0.25, 0.5)
+    want = a0 - lr * (mu * m + g * (0.5 / torch.linalg.vector_norm(g)))
+    assert float((a - want).abs().max()) < 1e-14
