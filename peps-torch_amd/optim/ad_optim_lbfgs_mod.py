@@ -158,11 +158,11 @@ def optimize_state(state, ctm_env_init, loss_fn, obs_fn=None, post_proc=None, ma
         t0 = time.perf_counter()
         loss.backward()
         parallel.average_grads(parameters)             # no-op in a single process; distributed runs: mean of the ranks' local gradients
+        t1 = time.perf_counter()
         if opt_args.opt_logging and opt_args.opt_log_grad:
             grad_log = [torch.view_as_real(p.grad).tolist() if p.grad.is_complex() else p.grad.tolist() for p in parameters]
         if clip > 0.0:
             raw_norms[0] = grads.clip_grad_norm_(parameters, clip).tolist()
-        t1 = time.perf_counter()
         current_env[0] = ctm_env.detach()
         _record(loss.item(), linesearching)
         if opt_args.opt_logging:

@@ -245,3 +245,51 @@ def test_a_run_resumes_from_a_checkpoint_of_torch_sgd(host, tmp_path, override):
     lr, mu = (0.125, 0.75) if override else (0.25, 0.5)
     want = a0 - lr * (mu * m + g * (0.5 / torch.linalg.vector_norm(g)))
     assert float((a - want).abs().max()) < 1e-14
+
+
+# ---- what the driver logs -------------------------------------------------------------------------------------------------------------------
+
+def test_time_of_the_gradient_is_that_of_the_backward_pass(host, tmp_path, monkeypatch):
+    """t_grad of the log line: neither the listing of the gradient (--OPTARGS_opt_log_grad) nor its norms."""
+    import logging
+    import json
+    import time
+    now = [0.0]
+    monkeypatch.setattr(time, "perf_counter", lambda: now[0])
+    tolist = torch.Tensor.tolist
+
+    def slow(t):
+        now[0] += 100.0
+        return tolist(t)
+    monkeypatch.setattr(torch.Tensor, "tolist", slow)
+    lines = []
+
+    class Lines(logging.Handler):
+        def emit(self, record):
+            lines.append(json.loads(record.getMessage()))
+    h = Lines()
+    L.log.addHandler(h)
+    try:
+        run(tmp_path, L, epochs=2, opt_log_grad=True, lr=0.5)
+    finally:
+        L.log.removeHandler(h)
+    lines = [l for l in lines if "t_grad" in l]
+    assert len(lines) == 2 and all(l["t_grad"] == 0.0 and len(l["grad"]) == 1 for l in lines)
+
+
+def test_another_optimiser_gets_the_scaled_gradient(host, tmp_path, monkeypatch):
+    """`create` of the driver: an optimiser that neither bounds its step itself nor is L-BFGS."""
+    from types import SimpleNamespace
+
+    def create(state, **kw):
+        ps = list(state.get_parameters())
+        for p in ps:
+            p.requires_grad_(True)
+        return ps, torch.optim.SGD(ps, lr=0.5)
+
+    def optimize_state(*a, **kw):
+        L.optimize_state(*a, create=create, **kw)
+    losses, mags, a, a0 = run(tmp_path, SimpleNamespace(optimize_state=optimize_state), epochs=1, clip_grad_norm=0.5, opt_log_grad=True)
+    g = a0 - 1.0
+    n = float(torch.linalg.vector_norm(g))
+    assert abs(mags[0][0] / n - 1.0) < 1e-14 and float((a - (a0 - 0.5 * 0.5 / n * g)).abs().max()) < 1e-14
