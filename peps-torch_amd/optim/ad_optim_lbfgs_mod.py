@@ -14,6 +14,7 @@ import time
 import torch
 import config as cfg
 import parallel
+from backend import get_engine
 from optim import grads
 
 log = logging.getLogger(__name__)
@@ -74,8 +75,9 @@ def load_optimizer_state_(optimizer, state, main_args=cfg.main_args, opt_args=cf
 
 def _grad_norms(gs):
     """[2-norm, largest modulus] of all gradients, on the host.  (Tensors that the engine does not take -- a run on an engine double on the
-    host, sites of different dtypes -- go through torch.)"""
-    if all(g.is_cuda and g.dtype is gs[0].dtype for g in gs) and gs[0].dtype in (torch.float64, torch.complex128):
+    host, sites of different dtypes, another device than the engine's -- go through torch.)"""
+    if all(g.is_cuda and g.dtype is gs[0].dtype and g.device == gs[0].device for g in gs) and gs[0].dtype in (torch.float64, torch.complex128) \
+            and getattr(get_engine(), "device", None) == gs[0].device:
         return grads.grad_norms(gs).tolist()
     flat = torch.cat(tuple(g.reshape(-1) for g in gs))
     return [flat.norm().item(), flat.abs().max().item()]

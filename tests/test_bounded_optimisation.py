@@ -293,3 +293,25 @@ def test_another_optimiser_gets_the_scaled_gradient(host, tmp_path, monkeypatch)
     g = a0 - 1.0
     n = float(torch.linalg.vector_norm(g))
     assert abs(mags[0][0] / n - 1.0) < 1e-14 and float((a - (a0 - 0.5 * 0.5 / n * g)).abs().max()) < 1e-14
+
+
+def test_gradients_that_the_engine_does_not_hold(monkeypatch):
+    """The log's norms of tensors on another device than the engine's go through torch, as those of host tensors do."""
+    import backend
+
+    class Elsewhere:
+        device = torch.device("cuda", 1)
+
+        def grad_norms(self, ts):
+            raise AssertionError("tensors of another device")
+
+    class OnGpu(torch.Tensor):                   # a host tensor that says it is on a device
+        is_cuda = property(lambda t: True)
+        device = property(lambda t: torch.device("cuda", 0))
+    g = t64(5).as_subclass(OnGpu)
+    backend.set_engine(Elsewhere())
+    try:
+        n2, top = L._grad_norms([g])
+    finally:
+        backend.set_engine(None)
+    assert abs(n2 / float(torch.linalg.vector_norm(t64(5))) - 1) < 1e-14 and top == float(t64(5).abs().max())
