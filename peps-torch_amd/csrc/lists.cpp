@@ -1,7 +1,8 @@
 // _ctm_lists: the short way from a Python list of tensors to the C entries over lists (ctm_grad_norms, ctm_grad_clip, ctm_sgd_step).  What those
 // entries cost on the lists of an optimisation is mostly the host's reading of pointers, dtypes and layouts: ten Python attribute accesses per
 // tensor are ~0.8 us, this module needs ~0.03 us.  It takes the plain case -- contiguous tensors of one dtype on one device -- and returns None for
-// everything else, refused arguments included (the interpreter's lock is held all along: nobody changes a list meanwhile); the caller (_native.py) then goes its general way, which handles strided views and words the errors.
+// everything else, refused arguments included (the interpreter's lock is held all along: nobody changes a list meanwhile); the caller (_native.py) then goes its
+// general way, which handles strided views and words the errors.
 #include <torch/csrc/Device.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
@@ -29,8 +30,9 @@ struct List {
     const at::Tensor& at(Py_ssize_t i) const { return THPVariable_Unpack(PySequence_Fast_GET_ITEM(seq, i)); }
 };
 
-// false: not the plain case.  `like`: the list whose shapes and dtype this one has to have.
-bool read(Call& c, PyObject* seq, List& l, const List* like) {
+// false: not the plain case.  `like`: the list whose shapes and dtype this one has to have.  `written`: the call writes it -- memory that a tensor
+// shares with its lazy clones until one of them is written becomes its own here.
+bool read(Call& c, PyObject* seq, List& l, const List* like, bool written) {
     if (!PyList_CheckExact(seq) && !PyTuple_CheckExact(seq)) return false;
     l.seq = seq;
     l.n = PySequence_Fast_GET_SIZE(seq);
@@ -47,7 +49,7 @@ bool read(Call& c, PyObject* seq, List& l, const List* like) {
         if (i == 0 && !like) c.cplx = st == at::kComplexDouble;
         if ((st == at::kComplexDouble) != c.cplx || !t.is_contiguous() || t.is_conj() || t.is_neg()) return false;
         if (like && t.sizes() != like->at(i).sizes()) return false;
-        l.ptr[i] = static_cast<const double*>(t.const_data_ptr());
+        l.ptr[i] = static_cast<const double*>(written ? t.mutable_data_ptr() : t.const_data_ptr());
         l.numel[i] = t.numel();
     }
     return c.context() != nullptr;
@@ -105,7 +107,7 @@ PyObject* general_way() {
 PyObject* grad_norms(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     ENTRY(6)
     List x;
-    if (read(c, a[5], x, nullptr)) {
+    if (read(c, a[5], x, nullptr, false)) {
         at::Tensor ws = workspace(c, x.n);
         const int st = ((norms_fn)c.fn)(c.context(), c.stream, (int)x.n, x.ptr.data(), x.numel.data(), ws.mutable_data_ptr<double>(), ws.numel());
         return st == CTM_OK ? norms_of(std::move(ws)) : failed(st);
@@ -117,7 +119,7 @@ PyObject* grad_norms(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 PyObject* grad_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     ENTRY(9)
     List x, y;
-    if (read(c, a[5], x, nullptr) && (a[6] == Py_None || read(c, a[6], y, &x))) {
+    if (read(c, a[5], x, nullptr, a[6] == Py_None) && (a[6] == Py_None || read(c, a[6], y, &x, true))) {
         const List& out = a[6] == Py_None ? x : y;
         const int code = (int)PyLong_AsLong(a[7]);
         const double bound = PyFloat_AsDouble(a[8]);
@@ -137,7 +139,7 @@ PyObject* sgd_step(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     ENTRY(14)
     List p, g, m;
     const bool buffers = a[7] != Py_None;
-    if (read(c, a[5], p, nullptr) && read(c, a[6], g, &p) && (!buffers || read(c, a[7], m, &p))) {
+    if (read(c, a[5], p, nullptr, true) && read(c, a[6], g, &p, false) && (!buffers || read(c, a[7], m, &p, true))) {
         const double lr = PyFloat_AsDouble(a[8]), mu = PyFloat_AsDouble(a[9]), tau = PyFloat_AsDouble(a[10]), bound = PyFloat_AsDouble(a[13]);
         const int first = PyObject_IsTrue(a[11]), code = (int)PyLong_AsLong(a[12]);
         if (PyErr_Occurred()) return nullptr;
