@@ -7,6 +7,7 @@ fallback: if the shared library is missing or a call fails, this module raises.
 import ctypes as C
 import os
 import threading
+import warnings
 os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")      # see config.py: one hardware queue per worker stream
 import torch
 
@@ -141,6 +142,15 @@ def load_lists():
     return _ctm_lists
 
 
+def _lists_or_none():
+    """load_lists(), or None and a warning: lists then go the general way (Engine._list) to the same kernels, everything else needs no module."""
+    try:
+        return load_lists()
+    except NativeError as e:
+        warnings.warn(str(e))
+        return None
+
+
 def _ptr(t):
     return C.c_void_p(t.data_ptr())
 
@@ -209,7 +219,7 @@ class Engine:
         self._options = {}
         self._tls = threading.local()          # the context selected by _bind is per CALLING THREAD (h, dtype below)
         self._create_lock = threading.Lock()
-        self._lists = load_lists()
+        self._lists = _lists_or_none()
         self._entries = {n: C.cast(getattr(self.lib, "ctm_" + n), C.c_void_p).value for n in ("grad_norms", "grad_clip", "sgd_step")}
         self.workers = []          # engines spawned for concurrent units (units.UnitPool): options/stats fan out to them
         self.default_cfg = TruncCfg(1e-8, 1e-8, 1e-14, 1, 1)

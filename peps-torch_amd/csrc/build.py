@@ -37,18 +37,26 @@ def asan_runtime():
 
 
 def build_ext(force=False, verbose=True):
-    deps = [EXT_SOURCE, os.path.join(HERE, "..", "..", "include", "ctm_hip.h")]
-    if not force and os.path.exists(EXT) and all(os.path.getmtime(EXT) >= os.path.getmtime(d) for d in deps):
-        return EXT
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ImportError:                       # the C library by itself needs neither torch nor this module
+        print("torch not found: _ctm_lists is not built", flush=True)
+        return None
+    deps = [EXT_SOURCE, os.path.join(HERE, "..", "..", "include", "ctm_hip.h")]
+    stamp, version = EXT + ".torch", str(torch.__version__)          # the release that it was compiled against
+    if not force and os.path.exists(EXT) and all(os.path.getmtime(EXT) >= os.path.getmtime(d) for d in deps) \
+            and os.path.exists(stamp) and open(stamp).read() == version:
+        return EXT
     root = os.path.dirname(torch.__file__)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DCTM_TORCH_VERSION="{version}"',
            "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I" + sysconfig.get_paths()["include"], EXT_SOURCE, "-o", EXT, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
+    with open(stamp, "w") as f:
+        f.write(version)
     return EXT
 
 

@@ -6,6 +6,7 @@
 #include <torch/csrc/Device.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <cstring>
 #include <vector>
 #include "../../include/ctm_hip.h"
 
@@ -165,4 +166,16 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ctm_lists", "Lists of tensors on 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__ctm_lists() { return PyModule_Create(&module); }
+// (the module reads torch's own structures: only with the release that it was compiled against)
+PyMODINIT_FUNC PyInit__ctm_lists() {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* version = torch ? PyObject_GetAttrString(torch, "__version__") : nullptr;
+    PyObject* str = version ? PyObject_Str(version) : nullptr;
+    const char* v = str ? PyUnicode_AsUTF8(str) : nullptr;
+    const bool same = v && !strcmp(v, CTM_TORCH_VERSION);
+    if (v && !same) PyErr_Format(PyExc_ImportError, "compiled against torch " CTM_TORCH_VERSION ", not %s", v);
+    Py_XDECREF(str);
+    Py_XDECREF(version);
+    Py_XDECREF(torch);
+    return same ? PyModule_Create(&module) : nullptr;
+}
