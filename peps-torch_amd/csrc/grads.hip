@@ -123,7 +123,8 @@ template <bool CPLX> __device__ __forceinline__ void add(Acc& a, d2 v) {
     } else {
         add_far(a, v.x);
         add_far(a, v.y);
-        if (CPLX) a.top_far = umax(a.top_far, bits(hypot(v.x, v.y)));
+        // (hypot of an infinity and a NaN is infinite)
+        if (CPLX) a.top_far = umax(a.top_far, bits(v.x != v.x || v.y != v.y ? __builtin_nan("") : hypot(v.x, v.y)));
     }
     if (!CPLX) { a.top = umax(a.top, bits(fabs(v.x))); a.top = umax(a.top, bits(fabs(v.y))); }
 }
