@@ -85,3 +85,25 @@ def test_bounded_lbfgs_over_several_epochs(eng, tmp_path, dtype):
         kw = dict(lr=0.75, epochs=8, max_iter_per_epoch=iters, tolerance_change=1e-9, tolerance_grad=1e-7)
         free, wide = run(tmp_path, L, "cuda", dtype, **kw), run(tmp_path, L, "cuda", dtype, clip_grad_norm=1e6, **kw)
         assert free[0] == wide[0] and torch.equal(free[2], wide[2]) and free[1] == wide[1]
+
+
+@pytest.mark.parametrize("dtype,n,bound", [(dt, n, b) for dt in (torch.float64, torch.complex128) for n in (3, 40, 12289) for b in (1e-3, 1e-10, 1e-300, 5e-324)]
+                         + [(torch.float64, 17000003, 1e-10)])
+def test_factors_below_the_normal_range(eng, dtype, n, bound):
+    """Norms near the largest double under an ordinary bound: c = bound / norm has no 53 bits left, the scaled list has."""
+    from test_gpu_grads import check_clip, check_norms, check_step, doubles, host, rand
+    import grads_oracle as O
+    rng = np.random.default_rng(12)
+    a = [rand(n, dtype, rng), rand(5, dtype, rng)]
+    a = [x * (1.5e308 / float(np.sqrt(sum((O.real_view(y) ** 2).sum() for y in a)))) for x in a]
+    t = [dev(x) for x in a]
+    out = [torch.zeros_like(x) for x in t]
+    for norm_type in (2, INF):
+        norms = check_norms(G.clip_grads(t, bound, norm_type, out=out), a)
+        check_clip(host(out), a, bound, norm_type, norms)
+    p0, m0 = [rand(x.shape, dtype, rng, bound) for x in a], [rand(x.shape, dtype, rng, bound) for x in a]
+    if bound < 1e-200:
+        return                                   # (sums of denormal numbers: exact or off by their own grid, nothing of the factor)
+    ps, ms = [dev(x) for x in p0], [dev(x) for x in m0]
+    G.sgd_step(ps, t, ms, lr=0.5, momentum=0.5, max_norm=bound)
+    check_step(host(ps), host(ms), p0, m0, a, O.factor(norms[0], bound), O.tol_n2(doubles(a)) + O.U, 0.5, 0.5, 0.0, False)
