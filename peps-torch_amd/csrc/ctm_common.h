@@ -58,10 +58,7 @@ struct Arena {
     int cur = -1;                  // current slab
     size_t top = 0;                // offset in the current slab
     size_t high = 0, total = 0;
-    std::vector<void*> guard_blocks;   // CTM_ARENA_GUARD=1 (diagnostic): every allocation its own hipMalloc, freed when its scope ends
 };
-extern int g_ctm_arena_guard;
-void arena_guard_release(struct ctm_ctx* ctx, size_t keep);
 
 // per-phase timers (seconds, host wall time with stream sync when profiling is enabled)
 enum { CTM_T_CORNERS = 0, CTM_T_HALVES, CTM_T_SVD, CTM_T_PROJ, CTM_T_ABSORB, CTM_T_NORM, CTM_T_RDM, CTM_T_EIG, CTM_T_COUNT };
@@ -260,9 +257,9 @@ int ctm_entry(ctm_ctx* ctx, const char* name, F&& body) {
 // arena API (ctm_runtime.hip)
 int arena_alloc(ctm_ctx* ctx, size_t bytes, void** out);
 struct ArenaScope {
-    ctm_ctx* c; int cur; size_t top; size_t nguard;
-    explicit ArenaScope(ctm_ctx* ctx) : c(ctx), cur(ctx->arena.cur), top(ctx->arena.top), nguard(ctx->arena.guard_blocks.size()) {}
-    ~ArenaScope() { c->arena.cur = cur; c->arena.top = top; if (c->arena.guard_blocks.size() > nguard) arena_guard_release(c, nguard); }
+    ctm_ctx* c; int cur; size_t top;
+    explicit ArenaScope(ctm_ctx* ctx) : c(ctx), cur(ctx->arena.cur), top(ctx->arena.top) {}
+    ~ArenaScope() { c->arena.cur = cur; c->arena.top = top; }
 };
 
 // event pair around a launch on ctx->stream while "gemm_timing" is on: begin returns the slot (or -1), end files it under `kind`

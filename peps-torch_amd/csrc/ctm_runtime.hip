@@ -64,31 +64,8 @@ void install_fatal_backtrace() {
 
 void ctm_note_launch(const char* kernel_name) { g_ring[g_ring_pos.fetch_add(1) % LAUNCH_RING] = kernel_name; }
 
-// CTM_ARENA_GUARD=1 (diagnostic, with tools/guard/guard_malloc.cpp preloaded): every arena allocation is its own hipMalloc of exactly
-// the requested size (16-byte granular), so a kernel that runs past the end of a workspace buffer faults instead of landing in its
-// neighbour on the stack; the blocks of a scope are freed (after a stream sync) when the scope ends.
-int g_ctm_arena_guard = [] { const char* e = getenv("CTM_ARENA_GUARD"); return (e && *e && *e != '0') ? 1 : 0; }();
-
-void arena_guard_release(ctm_ctx* ctx, size_t keep) {
-    (void)hipStreamSynchronize(ctx->stream);
-    Arena& a = ctx->arena;
-    while (a.guard_blocks.size() > keep) { (void)hipFree(a.guard_blocks.back()); a.guard_blocks.pop_back(); }
-}
-
 int arena_alloc(ctm_ctx* ctx, size_t bytes, void** out) {
     Arena& a = ctx->arena;
-    if (g_ctm_arena_guard) {
-        void* p = nullptr;
-        const size_t b = bytes ? (bytes + 15) & ~(size_t)15 : 16;
-        if (hipMalloc(&p, b) != hipSuccess) {
-            (void)hipGetLastError();
-            ctx->set_error("arena (guard mode): hipMalloc of " + std::to_string(b) + " bytes failed");
-            return CTM_ERR_NOMEM;
-        }
-        a.guard_blocks.push_back(p);
-        *out = p;
-        return CTM_OK;
-    }
     bytes = (bytes + 255) & ~(size_t)255;
     if (bytes == 0) bytes = 256;
     if (a.cur >= 0 && a.top + bytes <= a.slabs[a.cur].cap) {

@@ -17,8 +17,7 @@ def pytest_addoption(parser):
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
-    config.addinivalue_line("markers", "soak: long repeats / timing reports / out-of-scope script variants; deselected unless --soak or CTM_SOAK=1 "
-                                       "(tools/run_suite_original_order.sh passes --soak)")
+    config.addinivalue_line("markers", "soak: long repeats / timing reports / out-of-scope script variants; deselected unless --soak or CTM_SOAK=1")
 
 
 # Order of a `-m gpu` session: a session that is cut short (the driver's limit, a crash) must lose the LEAST important tests, and `-x` must

@@ -1,5 +1,5 @@
 // Scheduling probe (development tool, not product): does a chain of small latency-bound kernels make progress while chip-filling
-// kernels of another stream are resident?  Compares: plain streams, a high-priority stream for the chain, and CU-masked streams
+// kernels of another stream are resident?  Compares: plain streams and CU-masked streams
 // (hipExtStreamCreateWithCUMask: the chain on a few reserved CUs, the heavy stream on the complement).
 // build: hipcc --offload-arch=gfx950 -O2 tools/probe_cumask.hip -o tools/bin/probe_cumask
 #include <hip/hip_runtime.h>
@@ -123,13 +123,10 @@ int main(int argc, char** argv) {
         CK(hipStreamDestroy(s));
     };
     // ---- scheduling experiments
-    struct Cfg { const char* name; int nheavy; int light_mode; int reserve; };   // light_mode 0 plain, 1 high priority, 2 CU mask (reserve CUs), 3 mask + heavy unmasked
-    int lo, hi; CK(hipDeviceGetStreamPriorityRange(&lo, &hi));
-    printf("stream priority range: least %d greatest %d\n", lo, hi);
+    struct Cfg { const char* name; int nheavy; int light_mode; int reserve; };   // light_mode 0 plain, 2 CU mask (reserve CUs), 3 mask + heavy unmasked
     std::vector<Cfg> cfgs = {
         {"heavy alone, 1 stream", 1, -1, 0}, {"heavy alone, 2 streams", 2, -1, 0}, {"light alone", 0, 0, 0},
         {"1 heavy + light, plain", 1, 0, 0}, {"2 heavy + light, plain", 2, 0, 0},
-        {"1 heavy + light, high priority", 1, 1, 0}, {"2 heavy + light, high priority", 2, 1, 0},
         {"1 heavy(masked) + light on 8 reserved CUs", 1, 2, 8}, {"1 heavy(masked) + light on 16 reserved CUs", 1, 2, 16},
         {"2 heavy(masked) + light on 16 reserved CUs", 2, 2, 16}, {"2 heavy(masked) + light on 32 reserved CUs", 2, 2, 32},
         {"1 heavy(unmasked) + light masked to 16 CUs", 1, 3, 16},
@@ -151,7 +148,6 @@ int main(int argc, char** argv) {
             hs.push_back(s);
         }
         if (c.light_mode == 0) CK(hipStreamCreate(&ls));
-        else if (c.light_mode == 1) CK(hipStreamCreateWithPriority(&ls, hipStreamDefault, hi));
         else if (c.light_mode >= 2) ls = mask_stream(lm);
         Result r = run(hs, ls, c.nheavy ? HN : 0, ls ? LN : 0, heavy_wgs, heavy_lds, iters, light_wgs, light_lds, light_ns, dout, dwhere);
         printf("%-46s heavy %8.2f ms (%.3f per kernel per stream)   light chain %8.2f ms (%.1f us per link)\n", c.name, r.heavy_ms,
@@ -162,15 +158,12 @@ int main(int argc, char** argv) {
     // ---- heavy kernels with shorter-lived workgroups (4x the workgroups, 1/4 the work each): does the chain get in sooner?
     {
         std::vector<hipStream_t> hs(2); CK(hipStreamCreate(&hs[0])); CK(hipStreamCreate(&hs[1]));
-        hipStream_t ls; CK(hipStreamCreateWithPriority(&ls, hipStreamDefault, hi));
-        Result r = run(hs, ls, HN, LN, heavy_wgs * 4, heavy_lds, iters / 4, light_wgs, light_lds, light_ns, dout, dwhere);
-        printf("%-46s heavy %8.2f ms (%.3f per kernel per stream)   light chain %8.2f ms (%.1f us per link)\n", "2 heavy (3072 short wgs) + light high prio", r.heavy_ms, r.heavy_ms / HN, r.light_ms, 1e3 * r.light_ms / LN);
         hipStream_t lp; CK(hipStreamCreate(&lp));
-        r = run(hs, lp, HN, LN, heavy_wgs * 4, heavy_lds, iters / 4, light_wgs, light_lds, light_ns, dout, dwhere);
-        printf("%-46s heavy %8.2f ms (%.3f per kernel per stream)   light chain %8.2f ms (%.1f us per link)\n", "2 heavy (3072 short wgs) + light plain", r.heavy_ms, r.heavy_ms / HN, r.light_ms, 1e3 * r.light_ms / LN);
+        Result r = run(hs, lp, HN, LN, heavy_wgs * 4, heavy_lds, iters / 4, light_wgs, light_lds, light_ns, dout, dwhere);
+        printf("%-46s heavy %8.2f ms (%.3f per kernel per stream)   light chain %8.2f ms (%.1f us per link)\n", "2 heavy (short wgs) + light plain", r.heavy_ms, r.heavy_ms / HN, r.light_ms, 1e3 * r.light_ms / LN);
         // heavy kernels leaving LDS room: 2 per CU x 48 KB
-        r = run(hs, ls, HN, LN, 512, heavy_lds, iters * 3 / 2, light_wgs, light_lds, light_ns, dout, dwhere);
-        printf("%-46s heavy %8.2f ms (%.3f per kernel per stream)   light chain %8.2f ms (%.1f us per link)\n", "2 heavy (512 wgs: LDS room) + light high prio", r.heavy_ms, r.heavy_ms / HN, r.light_ms, 1e3 * r.light_ms / LN);
+        r = run(hs, lp, HN, LN, 512, heavy_lds, iters * 3 / 2, light_wgs, light_lds, light_ns, dout, dwhere);
+        printf("%-46s heavy %8.2f ms (%.3f per kernel per stream)   light chain %8.2f ms (%.1f us per link)\n", "2 heavy (512 wgs: LDS room) + light plain", r.heavy_ms, r.heavy_ms / HN, r.light_ms, 1e3 * r.light_ms / LN);
         // co-residency: heavy kernels that never fill a CU (2 x 48 KB of LDS, 8 of 32 wave slots) + light kernels that fit beside them (48 KB)
         std::vector<hipStream_t> h1{hs[0]};
         r = run(h1, lp, HN, LN, 512, heavy_lds, iters * 3 / 2, light_wgs, 48 * 1024, light_ns, dout, dwhere);
