@@ -15,7 +15,8 @@ HEADERS = ["ctm_common.h", "contract.h", "jacobi_internal.h", "grads_lists.h", o
 # Python module that reads lists of tensors (host code only, against torch's own headers)
 EXT_SOURCE = os.path.join(HERE, "lists.cpp")
 EXT = os.path.join(PKG, "_ctm_lists.so")
-# no packed single-precision arithmetic (v_pk_*_f32): some of its forms have given wrong results on this hardware
+# no packed single-precision arithmetic (v_pk_*_f32), which the compiler would make of float code by itself: kept out as a precaution (the kernels
+# compute in double precision, nothing here measures it)
 FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 LIB = os.path.join(PKG, "libctm_hip.so")
 LIB_ASAN = os.path.join(PKG, "libctm_hip_asan.so")

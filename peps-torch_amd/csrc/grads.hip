@@ -165,21 +165,27 @@ template <bool CPLX> __device__ __forceinline__ Part part_of(const Acc& a) {
 
 struct Bound { double max_norm; int inf_norm; };      // max_norm < 0: no bound
 
-// The factor as the kernels apply it: c = f s.  s = 1, but for c below the normal range (a norm above 2^1022 times the bound), where a double has
-// no 53 bits left for it: y = (x a / n) (max_norm / a), whose first product is at most a.  a = 4 keeps a / n normal, a = 1 the bits of a bound
-// that lies at the end of the range itself.
-struct Factor { double f, s; };
-__device__ __forceinline__ Factor factor_of(double n, double max_norm, double c) {
-    if (c < 0x1p-1022 && max_norm > 0.0 && n <= 0x1.fffffffffffffp1023) {
-        const double a = max_norm < 0x1p-1020 ? 1.0 : 4.0;
-        return {a / n, max_norm / a};
-    }
-    return {c, 1.0};
+// What the kernels multiply by: c itself, or, for a c below the normal range (a norm above 2^1022 times the bound), where a double has no 53 bits left
+// for it, -a / n: then y = (x a / n) (max_norm / a), whose first product is at most a.  a = 4 keeps a / n normal, a = 1 the bits of a bound that
+// lies at the end of the range itself.  (One double, whose sign tells which: two cost the step a wave per SIMD, 19.9 us against 19.6 on 61 MB.)
+__device__ __forceinline__ double tiny_a(double max_norm) { return max_norm < 0x1p-1020 ? 1.0 : 4.0; }
+__device__ __forceinline__ double multiplier(double n, double max_norm) {
+    const bool tiny = max_norm < n * 0x1p-1022 && max_norm > 0.0 && n <= 0x1.fffffffffffffp1023;
+    return (tiny ? -tiny_a(max_norm) : max_norm) / n;                                      // (NaN norm: NaN)
 }
-__device__ __forceinline__ d2 scaled(d2 x, Factor k) { return x * k.f * k.s; }
+template <int N> __device__ __forceinline__ void scale(d2 (&v)[N], double k, double max_norm) {
+    if (k < 0.0) {
+        const double s = max_norm / tiny_a(max_norm);
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = v[u] * -k * s;
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] *= k;
+    }
+}
 
-// N2, Ninf and the factor c from the three range sums
-struct Norms { double n2, ninf, c; Factor k; };
+// N2, Ninf and the multiplier from the three range sums
+struct Norms { double n2, ninf, k; };
 __device__ __forceinline__ Norms finish(const Part& p, Bound bd) {
     Norms r;
     if (p.big != 0.0) r.n2 = sqrt(fma(p.med * 0x1p-600, 0x1p-600, p.big)) * 0x1p600;
@@ -187,11 +193,15 @@ __device__ __forceinline__ Norms finish(const Part& p, Bound bd) {
     else r.n2 = sqrt(p.small) * 0x1p-600;
     r.ninf = __longlong_as_double((long long)p.top);
     const double n = bd.inf_norm ? r.ninf : r.n2;
-    r.c = (bd.max_norm < 0.0 || n <= bd.max_norm) ? 1.0 : bd.max_norm / n;      // NaN norm: NaN
-    r.k = factor_of(n, bd.max_norm, r.c);
+    r.k = (bd.max_norm < 0.0 || n <= bd.max_norm) ? 1.0 : multiplier(n, bd.max_norm);
     return r;
 }
-__device__ __forceinline__ void put_norms(const Norms& r, double* ws) { ws[0] = r.n2; ws[1] = r.ninf; ws[2] = r.c; }
+__device__ __forceinline__ void put_norms(const Norms& r, Bound bd, double* ws) {
+    ws[0] = r.n2;
+    ws[1] = r.ninf;
+    ws[2] = r.k < 0.0 ? bd.max_norm / (bd.inf_norm ? r.ninf : r.n2) : r.k;
+    ws[3] = r.k;
+}
 
 // First pass: partial results of the workgroups.
 template <bool CPLX, bool NT>
@@ -216,37 +226,36 @@ template <int T> __device__ __forceinline__ Norms join_partials(const Part* part
 
 __global__ __launch_bounds__(1024) void norm_finish_kernel(const Part* part, int np, Bound bd, double* ws) {
     const Norms r = join_partials<1024>(part, np, bd);
-    if (threadIdx.x == 0) put_norms(r, ws);
+    if (threadIdx.x == 0) put_norms(r, bd, ws);
 }
 
 // Where the second pass gets its factor from.  Lists of at most LONG chunks: every workgroup joins the partial results by itself (all get the same
 // bits) while its part of the list is on its way, which saves the 4 us of a kernel in between.  Longer ones, of many times more workgroups
 // than partial results: from ws, where norm_finish_kernel left it (np = 0).
 struct Source { const Part* part; int np; Bound bd; double* ws; bool write; };      // write: one workgroup leaves the norms in ws
-__device__ __forceinline__ Factor factor(const Source& s) {
-    if (s.bd.max_norm < 0.0) return {1.0, 1.0};
-    if (s.np == 0) return factor_of(s.ws[s.bd.inf_norm ? 1 : 0], s.bd.max_norm, s.ws[2]);
+__device__ __forceinline__ double factor(const Source& s) {
+    if (s.bd.max_norm < 0.0) return 1.0;
+    if (s.np == 0) return s.ws[3];
     const Norms r = join_partials<THREADS>(s.part, s.np, s.bd);
-    if (s.write && blockIdx.x == 0 && threadIdx.x == 0) put_norms(r, s.ws);
+    if (s.write && blockIdx.x == 0 && threadIdx.x == 0) put_norms(r, s.bd, s.ws);
     return r.k;
 }
 
 // y = c x (p[0] = x, p[1] = y).  In place a list inside the bound (c = 1) is neither read nor written.
 template <bool NT>
 __global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const Source s) {
-    Factor c{0.0, 1.0};
+    double k = 0.0;
     bool known = false;
     chunks<2>(t, [&](double* const* p, long long a, long long n) {
         d2 v[UNROLL];
         const bool apart = p[0] != p[1];
         if (apart) load_chunk<false>(v, p[0], a, n);
-        if (!known) { c = factor(s); known = true; }
+        if (!known) { k = factor(s); known = true; }
         if (!apart) {
-            if (c.f == 1.0 && c.s == 1.0) return;
+            if (k == 1.0) return;
             load_chunk<false>(v, p[0], a, n);
         }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) v[u] = scaled(v[u], c);
+        scale(v, k, s.bd.max_norm);
         store_chunk<NT>(v, p[1], a, n);
     });
 }
@@ -254,8 +263,7 @@ __global__ __launch_bounds__(THREADS) void clip_kernel(const Table<2> t, const S
 struct Step { double lr, mu, one_minus_tau; int first; };
 
 // d = c g -> the new momentum (MOMENTUM), p -> the new parameters
-template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d, d2 m, Factor c, const Step& s) {
-    d = scaled(d, c);
+template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d, d2 m, const Step& s) {
     if (MOMENTUM && !s.first) d = m * s.mu + d * s.one_minus_tau;
     p -= d * s.lr;
 }
@@ -263,16 +271,17 @@ template <bool MOMENTUM> __device__ __forceinline__ void step_pair(d2& p, d2& d,
 // p[0] = parameters, p[1] = gradients, p[2] = momentum buffers (MOMENTUM)
 template <bool MOMENTUM, bool NT>
 __global__ __launch_bounds__(THREADS) void sgd_kernel(const Table<MOMENTUM ? 3 : 2> t, const Step s, const Source src) {
-    Factor c{0.0, 1.0};
+    double k = 0.0;
     bool known = false;
     chunks<MOMENTUM ? 3 : 2>(t, [&](double* const* p, long long a, long long n) {
         d2 x[UNROLL], d[UNROLL], m[UNROLL];
         load_chunk<false>(d, p[1], a, n);
         if (MOMENTUM && !s.first) load_chunk<false>(m, p[MOMENTUM ? 2 : 0], a, n);
         load_chunk<false>(x, p[0], a, n);
-        if (!known) { c = factor(src); known = true; }
+        if (!known) { k = factor(src); known = true; }
+        scale(d, k, src.bd.max_norm);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) step_pair<MOMENTUM>(x[u], d[u], m[u], c, s);
+        for (int u = 0; u < UNROLL; ++u) step_pair<MOMENTUM>(x[u], d[u], m[u], s);
         if (MOMENTUM) store_chunk<NT>(d, p[MOMENTUM ? 2 : 0], a, n);
         store_chunk<NT>(x, p[0], a, n);
     });
@@ -323,8 +332,9 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(const Table<Shape<
     for (int r = 0; r < S::ROUNDS; ++r)
         if (wave + r * SMALL_WAVES < G) add<CPLX>(acc, v[r]);
     const Norms nr = finish(reduce_block<SMALL_WAVES>(part_of<CPLX>(acc)), bd);
-    if (threadIdx.x == 0) put_norms(nr, ws);
+    if (threadIdx.x == 0) put_norms(nr, bd, ws);
     if (OP == OP_NORMS) return;
+    scale(v, nr.k, bd.max_norm);
 #pragma unroll
     for (int r = 0; r < S::ROUNDS; ++r) {
         const unsigned q = wave + r * SMALL_WAVES;
@@ -332,9 +342,9 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(const Table<Shape<
         at.find(q, PIECE);
         const int i = (int)(q - at.f) * PIECE + 2 * lane, n = (int)at.n;
         if (OP == OP_CLIP) {
-            if (nr.c != 1.0 || at.p[S::NP - 1] != at.p[0]) store_piece(scaled(v[r], nr.k), at.p[S::NP - 1], i, n);
+            if (nr.k != 1.0 || at.p[S::NP - 1] != at.p[0]) store_piece(v[r], at.p[S::NP - 1], i, n);
         } else {
-            step_pair<OP == OP_SGD_MOMENTUM>(x[r], v[r], m[r], nr.k, s);
+            step_pair<OP == OP_SGD_MOMENTUM>(x[r], v[r], m[r], s);
             if (OP == OP_SGD_MOMENTUM) store_piece(v[r], at.p[S::NP - 1], i, n);
             store_piece(x[r], at.p[0], i, n);
         }

@@ -11,7 +11,7 @@ constexpr int THREADS = 256;
 constexpr int UNROLL = 4;              // 16-byte loads in flight per thread (545 MB: norms 87 us; 2: 97, 8: 91; 1.1 GB clipped 533; 2: 605, 8: 574)
 constexpr int CHUNK = 2 * THREADS * UNROLL;      // doubles: what a workgroup takes at a time; a chunk lies in one tensor
 constexpr int PIECE = 128;             // doubles: what a wave takes at a time in the one-workgroup kernels
-constexpr int WS_HEAD = 4;             // ws: N2, Ninf, c, unused, then the partial results (4 doubles each)
+constexpr int WS_HEAD = 4;             // ws: N2, Ninf, c, what the kernels multiply by, then the partial results (4 doubles each)
 constexpr int PARTIALS = 1024, PARTIALS_LEAST = 64;      // workgroups of the norm pass: over all launches, and of each launch besides (512: 94 us)
 
 // The tensors of one launch.  Their table travels by value in the kernel arguments (no host-to-device copy, so a call may be captured), which hold
