@@ -10,8 +10,9 @@ from optim import ad_optim_lbfgs_mod, grads
 class SGD(torch.optim.Optimizer):
     """torch.optim.SGD's iteration (lr, momentum, dampening) with the gradient scaled to 2-norm (or largest modulus, norm_type inf) at most `max_norm`
     over all parameters; `.grad` is not changed.  `norms` of the last step: device tensor [2-norm, largest modulus] of the raw gradient, None
-    without `max_norm`.  One parameter group, whose lr, momentum, dampening and max_norm may be changed between steps; a graph that captured
-    a step keeps those of the capture, and is captured after the first step (which makes the momentum buffers)."""
+    without `max_norm`.  One parameter group, of one dtype on the engine's device, whose lr, momentum, dampening and max_norm may be changed between
+    steps; a graph that captured a step keeps those of the capture, and is captured after the first step (which makes the momentum buffers).  A step
+    that raises leaves parameters and buffers as they were."""
 
     norms = None
 
