@@ -13,8 +13,9 @@ All tensors of a list are on the engine's device and of one dtype; empty tensors
 Tensors that are written share no memory with any other tensor of the call (clip_grads: but the one of the same index); where one of them is a
 strided view, two of them whose extents interleave (`m[:, :2]` and `m[:, 2:]`) are refused too.  A NaN anywhere, in one part of a complex element too, makes
 both norms NaN and a clipped list all NaN; a norm that is infinite or beyond the largest double makes c = 0 (0 x inf = NaN).  The returned norms are
-the head of the call's workspace, 35 kB and more: clone what is kept.  Calls run on the current stream, do not synchronise and may be captured into a graph (after one call outside of it, which makes the native context); they are not
-differentiable.  As every call of an engine they are one thread's at a time: another thread inside the same engine makes them raise NativeError."""
+the head of the call's workspace, 35 kB and more: clone what is kept.  Calls run on the current stream, do not synchronise and may be captured into a
+graph (after one call outside of it, which makes the native context); they are not differentiable.  As every call of an engine they are one thread's
+at a time: another thread inside the same engine makes them raise NativeError."""
 import torch
 from backend import get_engine
 

@@ -107,3 +107,17 @@ def test_factors_below_the_normal_range(eng, dtype, n, bound):
     ps, ms = [dev(x) for x in p0], [dev(x) for x in m0]
     G.sgd_step(ps, t, ms, lr=0.5, momentum=0.5, max_norm=bound)
     check_step(host(ps), host(ms), p0, m0, a, O.factor(norms[0], bound), O.tol_n2(doubles(a)) + O.U, 0.5, 0.5, 0.0, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.complex128])
+def test_without_the_module_that_reads_lists(eng, monkeypatch, dtype):
+    """The general way reaches the same kernels: the same bits."""
+    ts = [torch.randn(n, dtype=dtype, device="cuda") for n in (1, 513, 70001)]
+
+    def all_of_them():
+        p, m, x, o = ([t.clone() for t in ts] for _ in range(4))
+        r = [G.grad_norms(ts), G.clip_grads(x, 0.5), G.clip_grads(ts, 0.25, INF, out=o), G.sgd_step(p, ts, m, lr=0.5, momentum=0.5, max_norm=2.0)]
+        return torch.cat([torch.view_as_real(t).reshape(-1) if t.is_complex() else t for t in r + p + m + x + o])
+    short = all_of_them()
+    monkeypatch.setattr(eng, "_lists", None)
+    assert torch.equal(all_of_them(), short)
